@@ -69,6 +69,11 @@ PROTOTYPES = {
     "cfp_record_obs_soa": (C.c_int, [vp, vp, vp, vp, C.c_size_t, C.c_size_t, vp, vp, C.c_int, vp]),
     "cfp_record_obs_soa_list": (C.c_int, [vp, vp, vp, vp, C.c_size_t, C.c_size_t, vp, C.c_size_t,
                                           vp, C.c_int, vp, C.c_int, vp]),
+    "cfp_token_logprobs_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "cfp_token_logprobs": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, C.c_int, vp, vp, C.c_int64,
+                                     vp, vp, C.c_int, vp, vp, vp, vp, C.c_size_t, vp]),
+    "cfp_token_logprobs_grad": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, C.c_int, vp, vp,
+                                          C.c_int64, vp, vp, vp, C.c_int, vp, vp, vp, C.c_int64, vp]),
     "cfp_ppo_defaults": (C.c_int, [vp]),
     "cfp_train_create": (C.c_int, [C.POINTER(vp), vp, C.c_int, vp]),
     "cfp_train_destroy": (None, [vp]),

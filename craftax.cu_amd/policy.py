@@ -6,6 +6,7 @@ PyTorch is used only to own device memory and streams; every computation is a
 call into libcfpolicy.so.
 """
 import ctypes as C
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
@@ -497,6 +498,105 @@ def value_sample(av, seed, step_ctr=None, env_actions=None):
     _check(lib().cfp_value_sample(_ptr(av), n, w - 1, _ptr(env_actions), _ptr(act), _ptr(lp),
                                   _ptr(val), seed, _ptr(step_ctr), _stream()))
     return act, lp, val
+
+
+# -- log-probabilities of given tokens -------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum cfp_dtype
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _like(t, name, device, dtype, shape):
+    """An optional contiguous argument's pointer, checked."""
+    if t is None:
+        return None
+    _need(t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+          f"{name}: a contiguous {dtype} tensor {tuple(shape)} on {device} expected, "
+          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows_of(t, name):
+    """(pointer, dtype code, row stride) of a matrix whose rows are contiguous."""
+    _need(t.is_cuda and t.dim() == 2 and t.dtype in _DTYPES,
+          f"{name}: a [rows][vocab] fp32, bf16 or fp16 tensor on the GPU expected")
+    _need(t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1), f"{name}: rows must be contiguous")
+    return t.data_ptr(), _DTYPES[t.dtype], t.stride(0)
+
+
+def _mask_of(mask, device, rows, vocab):
+    """(pointer, row stride) of an optional mask: [rows][vocab] or [vocab], uint8 or bool."""
+    if mask is None:
+        return None, 0
+    _need(mask.device == device and mask.dtype in (torch.uint8, torch.bool) and
+          tuple(mask.shape) in ((rows, vocab), (vocab,)) and (vocab == 1 or mask.stride(-1) == 1),
+          f"mask: a uint8 or bool tensor ({rows}, {vocab}) or ({vocab},) with contiguous rows on {device} expected")
+    return mask.data_ptr(), mask.stride(0) if mask.dim() == 2 else 0
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results; top_* are None without alternatives, stats without `stats`."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+    stats: Optional[torch.Tensor]
+
+
+def token_logprobs(logits, tokens, mask=None, top=0, stats=False):
+    """ln p of given tokens (i32[rows]) under softmax(logits[rows][vocab]), the rows' entropies
+    and their `top` most probable entries (cfp_token_logprobs).  `logits` may be a view of wider
+    rows (the fused head's output without its value: av[:, :43]).  stats=True keeps what
+    token_logprobs_backward needs."""
+    ptr, dtype, ld = _rows_of(logits, "logits")
+    rows, vocab = logits.shape
+    dev = logits.device
+    tok = _like(tokens, "tokens", dev, torch.int32, (rows,))
+    _need(tok is not None, "tokens: expected")
+    mp, ldm = _mask_of(mask, dev, rows, vocab)
+    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top > 0 else None
+    tlp = torch.empty((rows, top), dtype=torch.float32, device=dev) if top > 0 else None
+    st = torch.empty((rows, 3), dtype=torch.float32, device=dev) if stats else None
+    need = lib().cfp_token_logprobs_workspace(rows, vocab, top)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with torch.cuda.device(dev):
+        _check(lib().cfp_token_logprobs(
+            ptr, dtype, ld, rows, vocab, tok, mp, ldm, lp.data_ptr(), ent.data_ptr(), top,
+            None if ids is None else ids.data_ptr(), None if tlp is None else tlp.data_ptr(),
+            None if st is None else st.data_ptr(), None if work is None else work.data_ptr(), need, _stream()))
+    return TokenLogprobs(lp, ent, ids, tlp, st)
+
+
+def token_logprobs_backward(logits, tokens, stats, g_logprobs=None, g_entropy=None, mask=None, top_ids=None,
+                            g_top=None, out=None):
+    """Gradient of the logits (their dtype) from the gradients of token_logprobs' results
+    (cfp_token_logprobs_grad).  out=logits replaces the logits."""
+    ptr, dtype, ld = _rows_of(logits, "logits")
+    rows, vocab = logits.shape
+    dev = logits.device
+    _need(stats is not None and tokens is not None, "tokens and the forward's stats: expected")
+    tok = _like(tokens, "tokens", dev, torch.int32, (rows,))
+    st = _like(stats, "stats", dev, torch.float32, (rows, 3))
+    g_lp = _like(g_logprobs, "g_logprobs", dev, torch.float32, (rows,))
+    g_ent = _like(g_entropy, "g_entropy", dev, torch.float32, (rows,))
+    mp, ldm = _mask_of(mask, dev, rows, vocab)
+    top = 0 if g_top is None else g_top.shape[-1]
+    _need(g_top is None or top_ids is not None, "g_top needs the forward's top_ids")
+    ids = _like(top_ids, "top_ids", dev, torch.int32, (rows, top)) if top else None
+    g_t = _like(g_top, "g_top", dev, torch.float32, (rows, top)) if top else None
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    _need(out.device == dev and out.dtype == logits.dtype and out.shape == logits.shape,
+          "out: the logits' shape, type and device expected")
+    op, _, ldo = _rows_of(out, "out")
+    with torch.cuda.device(dev):
+        _check(lib().cfp_token_logprobs_grad(ptr, dtype, ld, rows, vocab, tok, mp, ldm, st, g_lp, g_ent, top,
+                                             ids, g_t, op, ldo, _stream()))
+    return out
 
 
 def record_rd(rewards, terminals, r_reward_row, r_done_row):

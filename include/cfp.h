@@ -402,6 +402,48 @@ int cfp_value_sample(const float* d_av, int n, int actions, float* d_env_actions
 int cfp_record_rd(const float* d_rewards, const float* d_terminals, float* d_r_reward_row,
                   uint8_t* d_r_done_row, int n, void* stream);
 
+/* ---- log-probabilities of given tokens (csrc/token_logprobs.hip) ----------------
+ * No counterpart in the reference.  Beside cfp_value_sample: that draws an action from a
+ * row of at most 64 logits, these score tokens (actions) the caller already has, over rows
+ * of any width and of 16- or 32-bit logits, and give the gradient of the scores. */
+enum cfp_dtype { CFP_F32 = 0, CFP_BF16 = 1, CFP_F16 = 2 };
+/* Row r of d_logits (element type `dtype`, at r * ld elements) holds `vocab` logits.  An entry
+ * is allowed where its mask byte (d_mask + r * ld_mask, NULL = all ones; ld_mask 0 = the same
+ * mask for every row) is not 0 and its logit is above -inf; what stands in masked places, NaN
+ * included, is never used.  With p = softmax over the allowed entries, per row:
+ *   d_logprobs[r]     ln p[token]; 0 for a negative token (padding), -inf for one that is not
+ *                     allowed, NaN for one >= vocab
+ *   d_entropy[r]      -sum p ln p (NULL = not written)
+ *   d_top_ids / d_top_logprobs [r][top]   the `top` (0..32) largest allowed logits in
+ *                     descending order, equal ones by ascending index, and their ln p; places
+ *                     past the last allowed entry hold -1 and -inf
+ *   d_stats[r][3]     what cfp_token_logprobs_grad needs (NULL = not written)
+ * A row that allows nothing has log-probability -inf, entropy 0 and no alternatives; a row with
+ * NaN or +inf among its allowed logits has NaN and ids -1.  rows = 0 does nothing.
+ * Logits need the alignment of their type only.  ld >= vocab (any ld for one row).
+ * d_work: cfp_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte aligned (may be NULL
+ * where that is 0); calls that may overlap need one each. */
+size_t cfp_token_logprobs_workspace(int rows, int vocab, int top);
+int cfp_token_logprobs(const void* d_logits, int dtype, int64_t ld, int rows, int vocab,
+                       const int32_t* d_tokens, const uint8_t* d_mask, int64_t ld_mask,
+                       float* d_logprobs, float* d_entropy, int top, int32_t* d_top_ids,
+                       float* d_top_logprobs, float* d_stats, void* d_work, size_t work_bytes,
+                       void* stream);
+/* d_dlogits[r][v] (type `dtype`, row stride ld_dlogits) = the gradient of
+ *   sum_r g_logprobs[r] logprobs[r] + g_entropy[r] entropy[r] + sum_j g_top[r][j] top_logprobs[r][j]
+ * with respect to the logits, from the same logits, tokens and mask and the forward's d_stats
+ * (and d_top_ids where top > 0).  Each of d_g_logprobs, d_g_entropy may be NULL (= 0), and
+ * top = 0 leaves the alternatives out.  Entries that are not allowed get 0, and so does every
+ * entry of a row that allows nothing.  A log-probability that is the constant 0 or -inf passes
+ * no gradient on (negative or not allowed token, id -1); an index >= vocab makes the row's
+ * allowed entries NaN.  d_dlogits may be d_logits itself with the same stride (the logits are
+ * replaced); any other overlap is an error. */
+int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int rows, int vocab,
+                            const int32_t* d_tokens, const uint8_t* d_mask, int64_t ld_mask,
+                            const float* d_stats, const float* d_g_logprobs, const float* d_g_entropy,
+                            int top, const int32_t* d_top_ids, const float* d_g_top,
+                            void* d_dlogits, int64_t ld_dlogits, void* stream);
+
 /* ---- PPO update: replaces CuTrain (craftax_full.cu:12688-12761) ----------- */
 typedef struct cfp_trainer cfp_trainer;
 
