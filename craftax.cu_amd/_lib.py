@@ -74,6 +74,13 @@ PROTOTYPES = {
                                      vp, vp, C.c_int, vp, vp, vp, vp, C.c_size_t, vp]),
     "cfp_token_logprobs_grad": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int, C.c_int, vp, vp,
                                           C.c_int64, vp, vp, vp, C.c_int, vp, vp, vp, C.c_int64, vp]),
+    "cfp_orthogonalize_workspace": (C.c_size_t, [C.c_int]*4),
+    "cfp_orthogonalize": (C.c_int, [vp, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                    C.c_int, vp, C.c_float, C.c_int, vp, C.c_int64, C.c_int64, vp,
+                                    C.c_size_t, vp]),
+    "cfp_muon_update": (C.c_int, [vp, vp, vp, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, vp,
+                                  C.c_float, C.c_float, C.c_int, C.c_float, C.c_float, C.c_int, vp,
+                                  C.c_float, C.c_int, vp, C.c_size_t, vp]),
     "cfp_ppo_defaults": (C.c_int, [vp]),
     "cfp_train_create": (C.c_int, [C.POINTER(vp), vp, C.c_int, vp]),
     "cfp_train_destroy": (None, [vp]),

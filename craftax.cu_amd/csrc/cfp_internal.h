@@ -46,6 +46,28 @@ int value_sample(const float* d_av, int n, int actions, float* d_env_actions, in
 // records in recording mode on 32-env tiles, one tile per workgroup (at most one per CU).
 bool forward_draws(const FwdArgs& a);
 
+// One Muon step of a batch of fp32 matrices that share ld and stride (orthogonalize.hip,
+// cfp_muon_update); clear_g: the gradient is zeroed behind its last read.
+struct MuonArgs {
+    float* w;
+    float* g;
+    float* mom;
+    int64_t ld, stride;
+    int batch, rows, cols;
+    const float* lr_dev;   // or null: factor of lr in device memory
+    float lr, beta;
+    int nesterov;
+    float decay, scale;    // scale 0: sqrt(max(1, rows / cols))
+    int steps;
+    const float* coefs;    // host [steps][3] or null
+    float eps;
+    int products;          // 0 (= 3), 1 or 3
+    void* work;
+    size_t work_bytes;
+    int clear_g;
+};
+int muon_update(const MuonArgs& u, hipStream_t st);
+
 // One rollout step's policy side for the trainer: records -> heads into the policy's
 // live state and logits (r_state recorded), then the draw into act / logp / value
 // (and env_actions when not null) with offset *step_ctr, then *step_ctr += 1.  One

@@ -599,6 +599,71 @@ def token_logprobs_backward(logits, tokens, stats, g_logprobs=None, g_entropy=No
     return out
 
 
+# -- orthogonalised updates -------------------------------------------------------------
+def _matrices_of(t, name):
+    """(pointer, dtype code, ld, batch stride, batch, rows, cols) of [rows][cols] or [batch][rows][cols]."""
+    _need(t.is_cuda and t.dim() in (2, 3) and t.dtype in _DTYPES,
+          f"{name}: a [rows][cols] or [batch][rows][cols] fp32, bf16 or fp16 tensor on the GPU expected")
+    _need(t.shape[-2] > 0 and t.shape[-1] > 0 and (t.shape[-1] == 1 or t.stride(-1) == 1),
+          f"{name}: rows must be contiguous and not empty")
+    batch, stride = (t.shape[0], t.stride(0)) if t.dim() == 3 else (1, 0)
+    return t.data_ptr(), _DTYPES[t.dtype], t.stride(-2), stride, batch, t.shape[-2], t.shape[-1]
+
+
+def _coefs_of(coefs, steps):
+    """Host [steps][3] array of Newton-Schulz coefficients, or None for the standard ones."""
+    if coefs is None:
+        return None
+    a = np.ascontiguousarray(np.broadcast_to(np.asarray(coefs, dtype=np.float32), (steps, 3)))
+    return a
+
+
+def orthogonalize(g, steps=5, coefs=None, eps=1e-7, products=0, out=None):
+    """Newton-Schulz products towards the nearest semi-orthogonal matrix of each matrix of g
+    (cfp_orthogonalize).  coefs: (a, b, c) or one triple a step."""
+    ptr, dtype, ld, stride, batch, rows, cols = _matrices_of(g, "g")
+    dev = g.device
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    _need(out.shape == g.shape and out.dtype == g.dtype and out.device == dev,
+          "out: g's shape, type and device expected")
+    op, _, ldo, so, _, _, _ = _matrices_of(out, "out")
+    products = products or (1 if g.dtype == torch.bfloat16 else 3)
+    c = _coefs_of(coefs, steps)
+    need = lib().cfp_orthogonalize_workspace(batch, rows, cols, products)
+    work = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().cfp_orthogonalize(ptr, dtype, ld, stride, batch, rows, cols, steps,
+                                       None if c is None else c.ctypes.data, eps, products, op, ldo, so,
+                                       work.data_ptr(), need, _stream()))
+    return out
+
+
+def muon_update(w, g, momentum_buffer, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=0.0, steps=5,
+                coefs=None, eps=1e-7, products=0):
+    """One Muon step on fp32 weights w in place (cfp_muon_update); momentum_buffer is updated too.
+    lr: a number, or a one-element fp32 tensor on the GPU (read when the step runs)."""
+    ptr, dtype, ld, stride, batch, rows, cols = _matrices_of(w, "w")
+    dev = w.device
+    for t, name in ((g, "g"), (momentum_buffer, "momentum_buffer")):
+        _need(t.shape == w.shape and t.dtype == torch.float32 and w.dtype == torch.float32 and t.device == dev and
+              t.stride() == w.stride(), f"{name}: fp32 like w, with the same shape, strides and device, expected")
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        _need(lr.device == dev and lr.dtype == torch.float32 and lr.numel() == 1, "lr: one fp32 number on w's device")
+        lr, lr_dev = 1.0, lr.data_ptr()
+    products = products or 3
+    c = _coefs_of(coefs, steps)
+    need = lib().cfp_orthogonalize_workspace(batch, rows, cols, products)
+    work = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().cfp_muon_update(ptr, g.data_ptr(), momentum_buffer.data_ptr(), ld, stride, batch, rows, cols,
+                                     lr_dev, lr, momentum, 1 if nesterov else 0, weight_decay, scale, steps,
+                                     None if c is None else c.ctypes.data, eps, products, work.data_ptr(), need,
+                                     _stream()))
+    return w
+
+
 def record_rd(rewards, terminals, r_reward_row, r_done_row):
     _check(lib().cfp_record_rd(_ptr(rewards), _ptr(terminals), _ptr(r_reward_row),
                                _ptr(r_done_row), rewards.shape[0], _stream()))

@@ -444,6 +444,38 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
                             int top, const int32_t* d_top_ids, const float* d_g_top,
                             void* d_dlogits, int64_t ld_dlogits, void* stream);
 
+/* ---- orthogonalised updates (csrc/orthogonalize.hip) -------------------------------
+ * No counterpart in the reference (its optimiser is Adam, cfp_train_adam).  The nearest
+ * semi-orthogonal matrix of a gradient by Newton-Schulz products, as the Muon optimiser takes
+ * it: X = G / (|G|_F + eps), then `steps` (0..16) times, with the step's a, b, c,
+ *   A = X X^T,  B = b A + c A A,  X = a X + B X      (on the shorter side of G)
+ * d_g and d_out: `batch` matrices rows x cols (1..65536 each) of element type `dtype`, row
+ * strides ld / ld_out and matrix strides batch_stride / out_batch_stride in elements (any for a
+ * batch of one); d_out may be d_g.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315) for
+ * every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
+ * products: 1 = one fp16 matrix product per product (2e-3 of the result's norm from the 64-bit
+ * result), 3 = three (1e-6, as fp32), 0 = by type: 1 for bf16, 3 for fp32 and fp16.  Sums are
+ * fp32, the norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes all
+ * of it NaN.
+ * d_work: cfp_orthogonalize_workspace(batch, rows, cols, products) bytes (products 1 or 3),
+ * 256-byte aligned; calls that may overlap need one each. */
+size_t cfp_orthogonalize_workspace(int batch, int rows, int cols, int products);
+int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stride, int batch,
+                      int rows, int cols, int steps, const float* coefs, float eps, int products,
+                      void* d_out, int64_t ld_out, int64_t out_batch_stride, void* d_work,
+                      size_t work_bytes, void* stream);
+/* One Muon step of `batch` fp32 matrices w with gradients g and momentum buffers m (all with
+ * the same ld and batch_stride; g is left as it is):
+ *   m = momentum m + g,   u = g + momentum m (nesterov != 0) or m,   O = the above of u,
+ *   w = w (1 - lr weight_decay) - lr scale O
+ * lr is multiplied by *d_lr when that is not NULL (device memory: a captured step follows it).
+ * scale 0 = sqrt(max(1, rows / cols)).  products 0 = 3.  Workspace as above. */
+int cfp_muon_update(float* d_w, const float* d_g, float* d_momentum, int64_t ld,
+                    int64_t batch_stride, int batch, int rows, int cols, const float* d_lr, float lr,
+                    float momentum, int nesterov, float weight_decay, float scale, int steps,
+                    const float* coefs, float eps, int products, void* d_work, size_t work_bytes,
+                    void* stream);
+
 /* ---- PPO update: replaces CuTrain (craftax_full.cu:12688-12761) ----------- */
 typedef struct cfp_trainer cfp_trainer;
 

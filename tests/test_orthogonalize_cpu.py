@@ -1,0 +1,70 @@
+"""Argument checks of cfp_orthogonalize / cfp_muon_update: every refusal comes before the first
+HIP call, so none of this needs a GPU."""
+import ctypes as C
+
+import pytest
+
+P = C.c_void_p(0x10000)   # never dereferenced: each call below is refused on the host
+BIG = 1 << 40
+
+
+def _ortho(lib, g=P, dtype=0, ld=64, stride=64 * 64, batch=1, rows=64, cols=64, steps=5, eps=1e-7, products=0, out=P,
+           ldo=64, so=64 * 64, work=P, nbytes=BIG):
+    return lib.cfp_orthogonalize(g, dtype, ld, stride, batch, rows, cols, steps, None, eps, products, out, ldo, so,
+                                 work, nbytes, None)
+
+
+def _muon(lib, w=P, g=P, m=P, ld=64, stride=64 * 64, batch=1, rows=64, cols=64, steps=5, products=0, work=P, nbytes=BIG,
+          eps=1e-7):
+    return lib.cfp_muon_update(w, g, m, ld, stride, batch, rows, cols, None, 0.1, 0.9, 1, 0.0, 0.0, steps, None, eps,
+                               products, work, nbytes, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dtype=3), "dtype"), (dict(batch=-1), "batch"), (dict(batch=65536), "batch"), (dict(rows=0), "rows"),
+    (dict(cols=65537, ld=65537), "cols"), (dict(steps=17), "steps"), (dict(steps=-1), "steps"),
+    (dict(products=2), "products"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(g=None), "NULL"),
+    (dict(out=None), "NULL"), (dict(ld=63), "strides"), (dict(ldo=63), "strides"),
+    (dict(batch=2, stride=64 * 64 - 1), "overlap"), (dict(batch=2, so=0), "overlap"),
+    (dict(g=C.c_void_p(0x10002)), "aligned"), (dict(dtype=1, out=C.c_void_p(0x10001)), "aligned"),
+    (dict(work=None), "workspace"), (dict(nbytes=1000), "workspace"), (dict(work=C.c_void_p(0x10010)), "workspace"),
+])
+def test_orthogonalize_refuses(pkg, kw, word):
+    lib = pkg.lib()
+    assert _ortho(lib, **kw) != 0
+    assert word in lib.cfp_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(w=None), "NULL"), (dict(g=None), "NULL"), (dict(m=None), "NULL"), (dict(ld=10), "stride"),
+    (dict(batch=3, stride=9), "overlap"), (dict(steps=99), "steps"), (dict(products=5), "products"),
+    (dict(m=C.c_void_p(0x10002)), "aligned"), (dict(work=None), "workspace"), (dict(nbytes=1), "workspace"),
+    (dict(rows=1 << 17), "rows"), (dict(eps=-0.5), "eps"),
+])
+def test_muon_refuses(pkg, kw, word):
+    lib = pkg.lib()
+    assert _muon(lib, **kw) != 0
+    assert word in lib.cfp_last_error().decode()
+
+
+def test_no_matrices_is_no_work(pkg):
+    assert _ortho(pkg.lib(), batch=0, g=None, out=None, work=None, nbytes=0) == 0
+    assert _muon(pkg.lib(), batch=0, w=None, g=None, m=None, work=None, nbytes=0) == 0
+
+
+def test_workspace_sizes(pkg):
+    ws = pkg.lib().cfp_orthogonalize_workspace
+    assert ws(0, 64, 64, 1) == 0 and ws(1, 0, 64, 1) == 0 and ws(1, 64, 64, 2) == 0 and ws(1, 64, 1 << 17, 1) == 0
+    one, three = ws(1, 1000, 3000, 1), ws(1, 1000, 3000, 3)
+    # three matrices of the gradient's size and two of the shorter side squared, at least
+    assert one >= 2 * (3 * 1000 * 3000 + 2 * 1000 * 1000) and three > one
+    assert ws(1, 3000, 1000, 3) == three and ws(4, 1000, 3000, 3) > 3 * three
+    assert ws(1, 1 << 16, 1 << 16, 3) > 1 << 33     # sizes are not cut to 32 bits
+
+
+def test_python_checks_before_the_library(pkg):
+    import torch
+    with pytest.raises(ValueError, match="g:"):
+        pkg.policy.orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="w:"):
+        pkg.policy.muon_update(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), 0.1)
