@@ -23,7 +23,7 @@
 //          rounding of X at every step is amplified by a (3.44) a step where singular values
 //          are small: 5e-3 of the norm measured instead of 1 to 2e-3, which is a bf16 rounding
 //          (1.7e-3).  A third of the matrix instructions.  For bf16 inputs.
-#include <float.h>
+#include <utility>
 
 #include "cfp_internal.h"
 
@@ -32,16 +32,21 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 
 constexpr float kScaleX = 1024.0f, kScaleA = 256.0f;
 constexpr int kMaxSteps = 16;
-constexpr int kNormGroups = 64;   // partial sums of squares a matrix
+constexpr int kMaxNormGroups = 512;   // partial sums of squares a matrix
 
-// A row of a P = 3 matrix: blocks of 32 entries, the 32 hi parts then the 32 lo parts, so that
-// the 64 values of one LDS stage are one contiguous 128-byte piece either way.
+// Matrices are stored in pieces of 16 rows x 32 values, 1 KiB each and contiguous, the pieces of
+// 16 rows behind each other: a piece is what one wavefront copies to LDS with one instruction.
+// P = 3: the 32 values of a row are the hi parts of 16 entries, then their lo parts (kLo further).
+// ld: values a row, a multiple of 64.
+constexpr int kPiece = 512, kLo = 16;
 template <int P>
 __device__ __forceinline__ size_t at(size_t row, int ld, int k) {
-    return row * ld + (P == 3 ? (k >> 5) * 64 + (k & 31) : k);
+    const size_t piece = (row >> 4) * (size_t)(ld >> 5) + (P == 3 ? k >> 4 : k >> 5);
+    return piece * kPiece + (row & 15) * 32 + (P == 3 ? k & 15 : k & 31);
 }
 __device__ __forceinline__ void split_hl(float v, _Float16& hi, _Float16& lo) {
     hi = (_Float16)v;
@@ -55,40 +60,66 @@ struct InArgs {
     int dtype;
     int64_t ld, stride;
     int rows, cols;
+    int vec;             // rows start on four-element boundaries
     float* mom;          // or null; same ld and stride as g
     float beta;
     int nesterov;
     float* g_clear;      // or null: zeroed behind its last read
-    double* part;        // [batch][kNormGroups]
+    double* part;        // [batch][groups]
+    int groups;
     float eps;
 };
 __device__ __forceinline__ float load_any(const void* p, int dtype, size_t i) {
     return dtype == CFP_F32 ? ((const float*)p)[i]
                             : dtype == CFP_BF16 ? (float)((const __bf16*)p)[i] : (float)((const _Float16*)p)[i];
 }
+// four consecutive entries, the first `count` of which exist
+__device__ __forceinline__ f4 load_four(const void* p, int dtype, size_t i, int count, bool vec) {
+    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (vec && count >= 4) {
+        if (dtype == CFP_F32) return *reinterpret_cast<const f4*>((const float*)p + i);
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        if (dtype == CFP_BF16) return __builtin_convertvector(*reinterpret_cast<const b4*>((const __bf16*)p + i), f4);
+        return __builtin_convertvector(*reinterpret_cast<const h4*>((const _Float16*)p + i), f4);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < count) v[e] = load_any(p, dtype, i + e);
+    return v;
+}
+__device__ __forceinline__ void store_four(float* p, size_t i, int count, bool vec, const f4& v) {
+    if (vec && count >= 4) { *reinterpret_cast<f4*>(p + i) = v; return; }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < count) p[i + e] = v[e];
+}
 
 // First pass: momentum and the sum of squares (64 bits: squares of fp32 values neither
-// overflow nor vanish).
+// overflow nor vanish).  A wavefront takes 256 columns of a row at a time.
 __global__ __launch_bounds__(256) void k_ortho_norm(InArgs a) {
     __shared__ double ws[4];
     const size_t base = (size_t)blockIdx.y * a.stride;
+    const unsigned segs = (unsigned)(a.cols + 255) / 256, units = (unsigned)a.rows * segs;
+    const int lane = threadIdx.x & 63;
     double s = 0.0;
-    const int64_t total = (int64_t)a.rows * a.cols;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)kNormGroups * 256) {
-        const int r = (int)(e / a.cols), c = (int)(e - (int64_t)r * a.cols);
+    for (unsigned u = blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (unsigned)a.groups * 4) {
+        const unsigned r = u / segs;
+        const int c = (int)(u - r * segs) * 256 + 4 * lane, count = a.cols - c;
+        if (count <= 0) continue;
         const size_t i = base + (size_t)r * a.ld + c;
-        float u = load_any(a.g, a.dtype, i);
+        f4 v = load_four(a.g, a.dtype, i, count, a.vec);
         if (a.mom) {
-            const float m = a.beta * a.mom[i] + u;
-            a.mom[i] = m;
-            u = a.nesterov ? u + a.beta * m : m;
+            const f4 m = a.beta * load_four(a.mom, CFP_F32, i, count, a.vec) + v;
+            store_four(a.mom, i, count, a.vec, m);
+            v = a.nesterov ? v + a.beta * m : m;
         }
-        s += (double)u * (double)u;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s += (double)v[e] * (double)v[e];
     }
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
+    if (lane == 0) ws[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) a.part[(size_t)blockIdx.y * kNormGroups + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+    if (threadIdx.x == 0) a.part[(size_t)blockIdx.y * a.groups + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
 // The matrices of one call.  All live in the workspace, padded with zeros to whole tiles, which
@@ -96,63 +127,77 @@ __global__ __launch_bounds__(256) void k_ortho_norm(InArgs a) {
 struct Work {
     _Float16* x;        // [batch][mp][ldn]   X
     _Float16* y[2];     // [batch][np][ldm]   X transposed, before and after a step
-    _Float16* y_lo;     // [batch][np][mp]    P = 1: what X transposed lost in its rounding
+    _Float16* y_lo;     // [batch][np][ldm]   P = 1: what X transposed lost in its rounding
     _Float16* a;        // [batch][mp][ldm]
     _Float16* b;        // [batch][mp][ldm]
     int mp, np, ldm, ldn;
 };
 
-// Second pass: X = u / (|u| + eps) times kScaleX in both orders, zeros in the padding.
+// Second pass: X = u / (|u| + eps) times kScaleX in both orders, zeros in the padding.  A thread
+// takes four consecutive entries of four rows of a 64 x 64 tile, then of its transpose.
 template <int P>
 __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) {
     __shared__ float tile[64][65];
-    __shared__ float inv_s;
+    __shared__ double ws[4];
     const int bt = blockIdx.z;
-    if (threadIdx.x < 64) {
-        static_assert(kNormGroups == 64, "one partial sum a lane");
-        double s = a.part[(size_t)bt * kNormGroups + threadIdx.x];
-        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-        if (threadIdx.x == 0) inv_s = (float)((double)kScaleX / (sqrt(s) + (double)a.eps));
-    }
-    __syncthreads();
-    const float inv = inv_s;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < a.groups; i += 256) s += a.part[(size_t)bt * a.groups + i];
     const size_t base = (size_t)bt * a.stride;
     // G's rows and columns, padded
     const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;
+    const int x4 = 4 * (threadIdx.x & 15), y = threadIdx.x >> 4;
+    f4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int r = r0 + 16 * k + y, c = c0 + x4, count = r < a.rows ? a.cols - c : 0;
+        u[k] = load_four(a.g, a.dtype, base + (size_t)r * a.ld + c, count, a.vec);
+        if (a.mom) {
+            const f4 m = load_four(a.mom, CFP_F32, base + (size_t)r * a.ld + c, count, a.vec);
+            u[k] = a.nesterov ? u[k] + a.beta * m : m;
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
+    __syncthreads();
+    // in 64 bits: the reciprocal of a norm below 3e-36 is past fp32
+    const double norm = sqrt((ws[0] + ws[1]) + (ws[2] + ws[3])) + (double)a.eps;
+    const double inv = norm == 0.0 ? 0.0 : (double)kScaleX / norm;
     _Float16* d1 = tall ? w.y[0] + (size_t)bt * w.np * w.ldm : w.x + (size_t)bt * w.mp * w.ldn;
     _Float16* d2 = tall ? w.x + (size_t)bt * w.mp * w.ldn : w.y[0] + (size_t)bt * w.np * w.ldm;
     const int ld1 = tall ? w.ldm : w.ldn, ld2 = tall ? w.ldn : w.ldm;
-    _Float16* lo = P == 1 ? w.y_lo + (size_t)bt * w.np * w.mp : nullptr;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int i = ty; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + tx;
-        float u = 0.0f;
-        if (r < a.rows && c < a.cols) {
-            const size_t o = base + (size_t)r * a.ld + c;
-            u = load_any(a.g, a.dtype, o);
-            if (a.g_clear) a.g_clear[o] = 0.0f;
-            if (a.mom) {
-                const float m = a.mom[o];
-                u = a.nesterov ? u + a.beta * m : m;
-            }
-            u *= inv;
+    _Float16* lo = P == 1 ? w.y_lo + (size_t)bt * w.np * w.ldm : nullptr;
+    auto put = [&](_Float16* d, int ld, int r, int c, const f4& v, bool keep_lo) __attribute__((always_inline)) {
+        h4 hi, lw;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            _Float16 p, q;
+            split_hl(v[e], p, q);
+            hi[e] = p; lw[e] = q;
         }
-        tile[i][tx] = u;
-        _Float16 hi, lw;
-        split_hl(u, hi, lw);
-        const size_t o = at<P>(r, ld1, c);
-        d1[o] = hi;
-        if (P == 3) d1[o + 32] = lw;
-        if (P == 1 && tall) lo[(size_t)r * w.mp + c] = lw;
+        const size_t o = at<P>(r, ld, c);
+        *reinterpret_cast<h4*>(d + o) = hi;
+        if (P == 3) *reinterpret_cast<h4*>(d + o + kLo) = lw;
+        else if (keep_lo) *reinterpret_cast<h4*>(lo + o) = lw;
+    };
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int r = r0 + 16 * k + y, c = c0 + x4, count = r < a.rows ? a.cols - c : 0;
+        if (a.g_clear) store_four(a.g_clear, base + (size_t)r * a.ld + c, count, a.vec, f4{0.0f, 0.0f, 0.0f, 0.0f});
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = (float)((double)u[k][e] * inv);
+            tile[16 * k + y][x4 + e] = v[e];
+        }
+        put(d1, ld1, r, c, v, tall);
     }
     __syncthreads();
-    for (int i = ty; i < 64; i += 4) {
-        _Float16 hi, lw;
-        split_hl(tile[tx][i], hi, lw);
-        const size_t o = at<P>(c0 + i, ld2, r0 + tx);
-        d2[o] = hi;
-        if (P == 3) d2[o + 32] = lw;
-        if (P == 1 && !tall) lo[(size_t)(c0 + i) * w.mp + r0 + tx] = lw;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = tile[x4 + e][16 * k + y];
+        put(d2, ld2, c0 + 16 * k + y, r0 + x4, v, !tall);
     }
 }
 
@@ -181,6 +226,34 @@ __device__ __forceinline__ void put_out(const OutArgs& o, size_t i, float v) {
     }
 }
 
+// rows row0, row0 + 2, ... + 14, one column a lane
+__device__ __forceinline__ void put_rows(const OutArgs& o, size_t base, int row0, int col, const float (&v)[8]) {
+    if (col >= o.cols) return;
+    const size_t i = base + (size_t)row0 * o.ld + col, hop = 2 * (size_t)o.ld;
+    if (o.update) {
+        const float lr = o.lr_dev ? o.lr * *o.lr_dev : o.lr, keep = 1.0f - lr * o.decay, step = lr * o.scale;
+        float* w = (float*)o.out;
+        float old[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) old[k] = row0 + 2 * k < o.rows ? w[i + k * hop] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (row0 + 2 * k < o.rows) w[i + k * hop] = old[k] * keep - step * v[k];
+    } else if (o.dtype == CFP_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (row0 + 2 * k < o.rows) ((float*)o.out)[i + k * hop] = v[k];
+    } else if (o.dtype == CFP_BF16) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (row0 + 2 * k < o.rows) ((__bf16*)o.out)[i + k * hop] = (__bf16)v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (row0 + 2 * k < o.rows) ((_Float16*)o.out)[i + k * hop] = (_Float16)v[k];
+    }
+}
+
 // ---- the product C[i][j] = sum_k L[i][k] R[j][k] and what is made of it ---------------
 enum { kGram, kPoly, kStep, kLast };
 struct MulArgs {
@@ -188,8 +261,10 @@ struct MulArgs {
     const _Float16* r;
     int ldl, ldr;            // values (hi and lo counted apart) a row
     size_t l_batch, r_batch; // values a matrix
-    int stages;              // of 64 values
-    int tiles_i, tiles_j;
+    int stages;              // of 32 values; even
+    int tiles_i;
+    unsigned row_len;
+    uint64_t row_inv;
     Work w;
     int cur;                 // y[cur] is X transposed before the step
     float a, b, c;
@@ -199,190 +274,315 @@ __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// WM x WN wavefronts of FM x FN blocks of 32 x 32.  A stage is 64 values of every row of the
-// tile's L and R sides, 128 bytes a row, copied to LDS without registers (each lane's 16 bytes
-// land at the wave's base + 16 * lane) one stage ahead.  16-byte chunk c of row r sits at chunk
-// c ^ (r & 7): eight consecutive rows' fragments then cover all banks.
-template <int P, int MODE, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(64 * WM * WN) void k_ortho_mul(MulArgs g) {
-    constexpr int TM = 32 * WM * FM, TN = 32 * WN * FN, WAVES = WM * WN;
-    constexpr int LOADS = (TM + TN) / 8 / WAVES;   // 1 KiB pieces (8 rows) a wave
-    static_assert((TM / 8) % WAVES == 0 && (TN / 8) % WAVES == 0, "whole pieces a wave on either side");
-    __shared__ __align__(1024) unsigned char lds[2][(TM + TN) * 128];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
-    int ti, tj;
-    if (MODE == kGram || MODE == kPoly) {   // tiles on and above the diagonal, by columns
-        int t = (int)blockIdx.x;
-        tj = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-        while ((tj + 1) * (tj + 2) / 2 <= t) tj++;
-        while (tj * (tj + 1) / 2 > t) tj--;
-        ti = t - tj * (tj + 1) / 2;
+// Waits until at most min(later, MOST) * LOADS of this wave's copies are in flight.  Copies are
+// the only vector-memory operations between the prologue and the epilogue, so the counts are
+// those of the source.
+template <int LOADS, int MOST>
+__device__ __forceinline__ void wait_copies(int later) {
+    if (MOST >= 1 && later >= MOST) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * MOST) : "memory");
+    } else if constexpr (MOST > 1) {
+        wait_copies<LOADS, MOST - 1>(later);
     } else {
-        ti = (int)blockIdx.x % g.tiles_i;
-        tj = (int)blockIdx.x / g.tiles_i;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+}
+
+// Dwords 0, 1 of this lane and 2, 3 of lane - 32 (the lower half keeps 0, 1 and gets 0, 1 of lane
+// + 32 as its 2, 3): what turns 16 contiguous bytes of a row into the 8-byte pieces of two q, and
+// back.
+__device__ __forceinline__ void swap_halves(u4& v) {
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v[d], v[2 + d], false, false);
+        v[d] = r[0];
+        v[2 + d] = r[1];
+    }
+}
+__device__ __forceinline__ float half_of(const u4& v, int i) {
+    return (float)__builtin_bit_cast(h8, v)[i];
+}
+// Lane c of a quad holds entries (0..3, c) of a 4 x 4 matrix of fp16, two a dword; afterwards
+// entries (c, 0..3).
+__device__ __forceinline__ u2 transpose_quad(u2 w, int c) {
+    const unsigned sel = c & 1 ? 0x03020706u : 0x05040100u;   // odd: (other hi, own hi), even: (own lo, other lo)
+    u2 r;
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+        const unsigned other = __builtin_amdgcn_mov_dpp(w[d], 0xb1, 0xf, 0xf, true);   // lane ^ 1
+        r[d] = __builtin_amdgcn_perm(other, w[d], sel);
+    }
+    const bool low = (c & 2) == 0;
+    const unsigned got = __builtin_amdgcn_mov_dpp(low ? r[1] : r[0], 0x4e, 0xf, 0xf, true);   // lane ^ 2
+    return low ? u2{r[0], got} : u2{got, r[1]};
+}
+
+// f(0), f(1), ... with compile-time numbers (a loop of 48 steps is not unrolled whole)
+template <class Fn, int... I>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, Fn&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// 2 x 2 wavefronts of F x F blocks of 32 x 32 (tiles of 64 F).  A stage is SUB times 32 values of
+// every row of the tile's L and R sides, copied to LDS without registers (each lane's 16 bytes
+// land at the wave's base + 16 * lane) into a ring of R buffers.  16-byte chunk c of row r sits at
+// chunk c ^ (r / 4 & 3): the chunks of sixteen consecutive rows then cover all 64 banks.
+// A group is the matrix instructions of 16 of the K entries (P = 1: 32 values are two groups, P = 3:
+// one of three times as many); its operands are read from LDS while the group before it
+// multiplies, in an order that is pinned: left to itself the compiler reuses the operand registers
+// at once and waits for every read (615 instead of 1000 TFLOP/s at 4096 x 4096).
+template <int P, int MODE, int F, int SUB, int R>
+__global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
+    constexpr int T = 64 * F, WAVES = 4;
+    constexpr int LOADS = SUB * 2 * T / 16 / WAVES;   // pieces a wave and stage
+    constexpr int GROUPS = SUB * (P == 3 ? 1 : 2);
+    static_assert(GROUPS % 2 == 0 && LOADS % GROUPS == 0, "operand sets alternate; copies are spread evenly");
+    constexpr int PL = P == 3 ? 2 : 1;
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    constexpr int NM = (P == 3 ? 3 : 1) * F * F, NR = 2 * PL * F;
+    __shared__ __align__(1024) unsigned char lds[R][SUB][2 * T * 64];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+    // Tile of this workgroup; per_row is in scalar arithmetic throughout (addresses of copies are
+    // scalar operands): t / d as t * ceil(2^32 / d) / 2^32, exact while t * d < 2^32.
+    const unsigned t = blockIdx.x, row = (unsigned)((t * g.row_inv) >> 32), col = t - row * g.row_len;
+    int ti, tj;
+    if (MODE == kGram || MODE == kPoly) {
+        // tiles on and above the diagonal: row r and row n - 1 - r have n + 1 of them together
+        const int n = g.tiles_i, r = (int)row, c = (int)col;
+        ti = c < n - r ? r : n - 1 - r;
+        tj = c < n - r ? r + c : c - 1;
+    } else {
+        ti = (int)col;
+        tj = (int)row;
     }
     const size_t bt = blockIdx.y;
-    const int i0 = ti * TM, j0 = tj * TN;
-    const _Float16* lsrc = g.l + bt * g.l_batch + (size_t)i0 * g.ldl;
-    const _Float16* rsrc = g.r + bt * g.r_batch + (size_t)j0 * g.ldr;
-
-    const int prow = lane >> 3, pchunk = (lane & 7) ^ (prow & 7);
-    auto copy_stage = [&](int s, int buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int q = 0; q < LOADS; q++) {
-            constexpr int LL = TM / 8 / WAVES;   // the first LL pieces are of the L side
-            const int piece = (q < LL ? q : q - LL) * WAVES + wave;
-            const _Float16* src = q < LL ? lsrc : rsrc;
-            const int ld = q < LL ? g.ldl : g.ldr;
-            const _Float16* from = src + (size_t)piece * 8 * ld + (size_t)s * 64;   // uniform
-            const unsigned voff = (unsigned)(prow * ld * 2 + pchunk * 16);
-            const unsigned to = (unsigned)(size_t)&lds[buf][((q < LL ? 0 : TM) + piece * 8) * 128];
-            asm volatile(
-                "s_mov_b32 m0, %2\n\t"
-                "s_nop 0\n\t"
-                "global_load_lds_dwordx4 %0, %1"
-                :
-                : "v"(voff), "s"(from), "s"(to)
-                : "memory", "m0");
-        }
+    const int i0 = ti * T, j0 = tj * T;
+    // this wave's pieces of stage 0: F of the L side, F of the R side
+    const _Float16* from[2] = {g.l + bt * g.l_batch + (size_t)(i0 / 16 + wave) * (g.ldl >> 5) * kPiece,
+                               g.r + bt * g.r_batch + (size_t)(j0 / 16 + wave) * (g.ldr >> 5) * kPiece};
+    const size_t hop[2] = {(size_t)WAVES * (g.ldl >> 5) * kPiece, (size_t)WAVES * (g.ldr >> 5) * kPiece};
+    const unsigned voff = (unsigned)((lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16);
+    // copy q of a stage into ring buffer `buf`: sub-stage by sub-stage, the L side first
+    auto copy = [&](int stage, int buf, int q) __attribute__((always_inline)) {
+        constexpr int HALF = LOADS / SUB / 2;
+        const int sub = q / (2 * HALF), side = q / HALF % 2, i = q % HALF;
+        const unsigned to = (unsigned)(size_t)&lds[buf][sub][(side * T + (i * WAVES + wave) * 16) * 64];
+        asm volatile(
+            "s_mov_b32 m0, %2\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %0, %1"
+            :
+            : "v"(voff + (unsigned)(stage * SUB + sub) * (kPiece * 2)), "s"(from[side] + i * hop[side]), "s"(to)
+            : "memory", "m0");
     };
 
-    f16v acc[FM][FN];
+    // F = 1 has one block a wavefront: products of different planes or K steps go to accumulators
+    // of their own, or each matrix instruction would wait for the one before it.
+    constexpr int ACCS = F > 1 ? 1 : P == 3 ? 3 : 2;
+    f16v acc[F][F][ACCS];
 #pragma unroll
-    for (int i = 0; i < FM; i++)
+    for (int i = 0; i < F * F * ACCS; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-    const int wi = (wave % WM) * FM * 32, wj = (wave / WM) * FN * 32;
-    auto frag = [&](int buf, int row, int chunk) __attribute__((always_inline)) {
-        return *reinterpret_cast<const h8*>(&lds[buf][row * 128 + ((chunk ^ (row & 7)) * 16)]);
+        for (int e = 0; e < 16; e++) acc[i / (F * ACCS)][i / ACCS % F][i % ACCS][e] = 0.0f;
+    const int wi = (wave & 1) * F * 32, wj = (wave >> 1) * F * 32;
+    // operand registers of two groups: [group][plane][side][block]
+    h8 op[2][PL][2][F];
+    const int chunk_of[2] = {(half ^ ((n32 >> 2) & 3)) * 16, ((2 + half) ^ ((n32 >> 2) & 3)) * 16};
+    // operand t of group `gr` of the stage in buffer `buf`, in the order of use: the hi planes
+    // first, L and R in turn
+    auto read = [&](int buf, int gr, int t) __attribute__((always_inline)) {
+        const int sub = P == 3 ? gr : gr / 2, z = t / (2 * F), side = t % 2, b = (t % (2 * F)) / 2;
+        const int row = side * T + (side ? wj : wi) + 32 * b + n32;
+        op[gr % 2][z][side][b] = *reinterpret_cast<const h8*>(&lds[buf][sub][row * 64 + chunk_of[P == 3 ? z : gr % 2]]);
     };
-    copy_stage(0, 0);
-    for (int s = 0; s < g.stages; s++) {
-        // this wave's pieces of stage s have landed; behind the barrier everyone's have, and
-        // nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto multiply = [&](int gr, int m) __attribute__((always_inline)) {
+        const int z = m / (F * F), i = (m % (F * F)) / F, j = m % F;   // z: hi hi, hi lo, lo hi
+        f16v& to = acc[i][j][ACCS == 1 ? 0 : P == 3 ? z : gr % 2];
+        to = mma(op[gr % 2][z == 2 ? PL - 1 : 0][0][i], op[gr % 2][z == 1 ? PL - 1 : 0][1][j], to);
+    };
+    // Group `gr`: its matrix instructions, one LDS read of the next group's operands (next_buf)
+    // behind each of the first ones, and its share of the copies of stage `stage` into buffer
+    // `free_buf` spread over it (a burst of copies fills the address unit's queue and stops the
+    // wave).
+    auto group = [&](auto at_gr, auto reading, auto copying, int next_buf, int stage, int free_buf, int share)
+                     __attribute__((always_inline)) {
+        constexpr int gr = decltype(at_gr)::value, next = (gr + 1) % GROUPS, Q = LOADS / GROUPS;
+        __builtin_amdgcn_sched_barrier(0);
+        each(std::make_integer_sequence<int, NM>{}, [&](auto at_m) __attribute__((always_inline)) {
+            constexpr int m = decltype(at_m)::value;
+            multiply(gr, m);
+            if (decltype(reading)::value)
+#pragma unroll
+                for (int t = m * NR / NM; t < (m + 1) * NR / NM; t++) read(next_buf, next, t);
+            if (decltype(copying)::value)
+#pragma unroll
+                for (int q = m * Q / NM; q < (m + 1) * Q / NM; q++) copy(stage, free_buf, share * Q + q);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    using std::integral_constant;
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    // Stage s from its last group on to the last but one of stage s + 1.  Before that group reads
+    // stage s + 1: this wave's copies of it have landed, behind the barrier everyone's have; and
+    // everyone has read all of stage s, whose buffer takes stage s + R.
+    auto advance = [&](auto copying, int s, int buf, int nb, int later) __attribute__((always_inline)) {
+        wait_copies<LOADS, R - 2>(later);
         __syncthreads();
-        const int buf = s & 1;
-        if (s + 1 < g.stages) copy_stage(s + 1, buf ^ 1);
-        if (P == 1) {
+        group(integral_constant<int, GROUPS - 1>{}, yes, copying, nb, s + R, buf, 0);
+        each(std::make_integer_sequence<int, GROUPS - 1>{}, [&](auto at) __attribute__((always_inline)) {
+            group(at, yes, copying, nb, s + R, buf, decltype(at)::value + 1);
+        });
+    };
+    const int last = g.stages / SUB - 1;
+    for (int s = 0; s < R && s <= last; s++)
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                h8 l[FM], r[FN];
+        for (int q = 0; q < LOADS; q++) copy(s, s, q);
+    wait_copies<LOADS, R - 1>(last);
+    __syncthreads();
 #pragma unroll
-                for (int i = 0; i < FM; i++) l[i] = frag(buf, wi + 32 * i + n32, 2 * ks + half);
-#pragma unroll
-                for (int j = 0; j < FN; j++) r[j] = frag(buf, TM + wj + 32 * j + n32, 2 * ks + half);
-#pragma unroll
-                for (int i = 0; i < FM; i++)
-#pragma unroll
-                    for (int j = 0; j < FN; j++) acc[i][j] = mma(l[i], r[j], acc[i][j]);
-            }
-        } else {
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                h8 l[2][FM], r[2][FN];
-#pragma unroll
-                for (int z = 0; z < 2; z++) {
-#pragma unroll
-                    for (int i = 0; i < FM; i++) l[z][i] = frag(buf, wi + 32 * i + n32, 4 * z + 2 * ks + half);
-#pragma unroll
-                    for (int j = 0; j < FN; j++) r[z][j] = frag(buf, TM + wj + 32 * j + n32, 4 * z + 2 * ks + half);
-                }
-#pragma unroll
-                for (int z = 0; z < 3; z++)   // hi hi, hi lo, lo hi
-#pragma unroll
-                    for (int i = 0; i < FM; i++)
-#pragma unroll
-                        for (int j = 0; j < FN; j++)
-                            acc[i][j] = mma(l[z == 2][i], r[z == 1][j], acc[i][j]);
-            }
-        }
+    for (int t = 0; t < NR; t++) read(0, 0, t);
+    each(std::make_integer_sequence<int, GROUPS - 1>{}, [&](auto at) __attribute__((always_inline)) {
+        group(at, yes, no, 0, 0, 0, 0);
+    });
+    int buf = 0, s = 0;
+    for (; s + R <= last; s++) {
+        const int nb = buf == R - 1 ? 0 : buf + 1;
+        advance(yes, s, buf, nb, R - 2);
+        buf = nb;
     }
+    for (; s < last; s++) {
+        const int nb = buf == R - 1 ? 0 : buf + 1;
+        advance(no, s, buf, nb, last - s - 1);
+        buf = nb;
+    }
+    group(integral_constant<int, GROUPS - 1>{}, no, no, 0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < F * F; i++)
+#pragma unroll
+        for (int z = 1; z < ACCS; z++) acc[i / F][i % F][0] += acc[i / F][i % F][z];
 
-    // Lane's part of a block: column n32, rows 8 q + 4 half + 0..3 (q = 0..3), so four
-    // consecutive entries of a row of the transposed matrix.
+    // ---- epilogue.  A lane holds column n32 of a block, rows 8 q + 4 half + 0..3 (q = 0..3).
+    // Transposed matrices (rows j) are read and written 16 bytes a lane: lanes n32 and n32 + 32
+    // hold neighbouring 8-byte pieces, of q = 2 t and 2 t + 1, and swap two of the four dwords.
+    // The last step's values leave through LDS, a block column of the wavefront at a time: whole
+    // rows of the result in either order.  Its operands are read (barrier).
+    float (*out_stage)[32][33] = reinterpret_cast<float (*)[32][33]>(&lds[0][0][0] + wave * (F * 32 * 33 * 4));
+    static_assert(sizeof(lds) >= 4 * F * 32 * 33 * 4, "the stage of the results fits into the ring");
+    if (MODE == kLast) __syncthreads();
+    const int end_i = g.w.mp, end_j = SYM ? g.w.mp : g.w.np;
+    const int quad = lane & 3;
+    const size_t mat_a = bt * g.w.mp * (size_t)g.w.ldm, mat_y = bt * g.w.np * (size_t)g.w.ldm;
+    // what is added to the product: X transposed (with its lo part), or A
+    const _Float16* addend = MODE == kGram ? nullptr : MODE == kPoly ? g.w.a + mat_a : g.w.y[g.cur] + mat_y;
+    constexpr bool HAS_LO = P == 3 || !SYM;
 #pragma unroll
-    for (int fi = 0; fi < FM; fi++)
+    for (int fj = 0; fj < F; fj++) {
+        const int jb = j0 + wj + 32 * fj, j = jb + n32;
+        if (jb >= end_j) continue;   // whole blocks: the ends are multiples of 64
+        u4 add[F][2][2];   // [block][t][hi, lo]; the loads of BATCH blocks are in flight together
+        constexpr int BATCH = F == 4 ? (P == 3 ? 1 : 2) : F;   // more do not fit beside 256 accumulators
 #pragma unroll
-        for (int fj = 0; fj < FN; fj++)
+        for (int f0 = 0; f0 < F; f0 += BATCH) {
+        if (MODE != kGram)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int i = i0 + wi + 32 * fi + 8 * q + 4 * half, j = j0 + wj + 32 * fj + n32;
-                float v[4];
+            for (int fi = f0; fi < f0 + BATCH; fi++) {
+                const int ib = i0 + wi + 32 * fi;
+                if (ib >= end_i) continue;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[fi][fj][4 * q + e];
-                if (MODE == kGram || MODE == kPoly) {
-                    _Float16* m = (MODE == kGram ? g.w.a : g.w.b) + bt * g.w.mp * (size_t)g.w.ldm;
-                    const size_t across = at<P>(j, g.w.ldm, i);
-                    if (MODE == kGram) {
+                for (int t = 0; t < 2; t++) {
+                    const _Float16* from_y = addend + at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
+                    add[fi][t][0] = *reinterpret_cast<const u4*>(from_y);
+                    if (P == 3) add[fi][t][1] = *reinterpret_cast<const u4*>(from_y + kLo);
+                    else if (HAS_LO) add[fi][t][1] = *reinterpret_cast<const u4*>(g.w.y_lo + mat_y + at<1>(j, g.w.ldm, ib + 16 * t) + 8 * half);
+                }
+            }
 #pragma unroll
-                        for (int e = 0; e < 4; e++) v[e] *= kScaleA / (kScaleX * kScaleX);
-                    } else {
-                        const _Float16* am = g.w.a + bt * g.w.mp * (size_t)g.w.ldm;
-                        const h4 hi = *reinterpret_cast<const h4*>(am + across);
-                        h4 lo{};
-                        if (P == 3) lo = *reinterpret_cast<const h4*>(am + across + 32);
+        for (int fi = f0; fi < f0 + BATCH; fi++) {
+            const int ib = i0 + wi + 32 * fi;
+            if (ib >= end_i) continue;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if (MODE != kGram) {
+                    swap_halves(add[fi][t][0]);
+                    if (HAS_LO) swap_halves(add[fi][t][1]);
+                }
+                u4 hi_out, lo_out;   // dwords 0, 1: q = 2 t; 2, 3: q = 2 t + 1
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int q = 2 * t + u;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = acc[fi][fj][0][4 * q + e];
+                        float x = 0.0f;
+                        if (MODE != kGram) {
+                            x = half_of(add[fi][t][0], 4 * u + e);
+                            if (HAS_LO) x += half_of(add[fi][t][1], 4 * u + e);
+                        }
+                        if (MODE == kGram) v[e] *= kScaleA / (kScaleX * kScaleX);
+                        else if (MODE == kPoly) v[e] = g.b * x + (g.c / kScaleA) * v[e];
+                        else v[e] = g.a * x + v[e] * (1.0f / kScaleA);
+                    }
+                    if (MODE == kLast) {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            v[e] = g.b * ((float)hi[e] + (float)lo[e]) + (g.c / kScaleA) * v[e];
+                            out_stage[fi][8 * q + 4 * half + e][n32] = v[e] * (1.0f / kScaleX);
+                        continue;
                     }
                     h4 hi, lo;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        _Float16 x, y;
-                        split_hl(v[e], x, y);
-                        hi[e] = x; lo[e] = y;
+                        _Float16 p, r;
+                        split_hl(v[e], p, r);
+                        hi[e] = p; lo[e] = r;
                     }
-                    // a tile on the diagonal holds both halves itself, and stores one of them
-                    if (ti != tj) {
-                        *reinterpret_cast<h4*>(m + across) = hi;
-                        if (P == 3) *reinterpret_cast<h4*>(m + across + 32) = lo;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const size_t o = at<P>(i + e, g.w.ldm, j);
-                        m[o] = hi[e];
-                        if (P == 3) m[o + 32] = lo[e];
-                    }
-                } else {
-                    const _Float16* y = g.w.y[g.cur] + bt * g.w.np * (size_t)g.w.ldm;
-                    const size_t o = at<P>(j, g.w.ldm, i);
-                    _Float16* ylo = P == 1 ? g.w.y_lo + (bt * g.w.np + j) * g.w.mp + i : nullptr;
-                    const h4 xh = *reinterpret_cast<const h4*>(y + o);
-                    const h4 xl = *reinterpret_cast<const h4*>(P == 3 ? y + o + 32 : ylo);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = g.a * ((float)xh[e] + (float)xl[e]) + v[e] * (1.0f / kScaleA);
-                    if (MODE == kLast) {
-                        const OutArgs& t = g.out;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int row = t.tall ? j : i + e, col = t.tall ? i + e : j;
-                            if (row < t.rows && col < t.cols)
-                                put_out(t, bt * t.stride + (size_t)row * t.ld + col, v[e] * (1.0f / kScaleX));
-                        }
-                    } else {
-                        h4 hi, lo;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            _Float16 p, r;
-                            split_hl(v[e], p, r);
-                            hi[e] = p; lo[e] = r;
-                        }
-                        _Float16* yn = g.w.y[g.cur ^ 1] + bt * g.w.np * (size_t)g.w.ldm;
-                        *reinterpret_cast<h4*>(yn + o) = hi;
-                        *reinterpret_cast<h4*>(P == 3 ? yn + o + 32 : ylo) = lo;
-                        _Float16* x = g.w.x + bt * g.w.mp * (size_t)g.w.ldn;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const size_t ox = at<P>(i + e, g.w.ldn, j);
-                            x[ox] = hi[e];
-                            if (P == 3) x[ox + 32] = lo[e];
-                        }
-                    }
+                    const u2 hw = __builtin_bit_cast(u2, hi), lw = __builtin_bit_cast(u2, lo);
+                    hi_out[2 * u] = hw[0]; hi_out[2 * u + 1] = hw[1];
+                    lo_out[2 * u] = lw[0]; lo_out[2 * u + 1] = lw[1];
+                    // row-major: four lanes exchange their columns, one row of four entries each
+                    _Float16* to = MODE == kGram ? g.w.a + mat_a : MODE == kPoly ? g.w.b + mat_a
+                                                                                 : g.w.x + bt * g.w.mp * (size_t)g.w.ldn;
+                    to += at<P>(ib + 8 * q + 4 * half + quad, SYM ? g.w.ldm : g.w.ldn, jb + (n32 & 28));
+                    *reinterpret_cast<u2*>(to) = transpose_quad(hw, quad);
+                    if (P == 3) *reinterpret_cast<u2*>(to + kLo) = transpose_quad(lw, quad);
+                }
+                if (MODE == kLast) continue;
+                // a tile on the diagonal holds both halves itself, and has stored them
+                if (SYM && ti == tj) continue;
+                _Float16* to = SYM ? (MODE == kGram ? g.w.a : g.w.b) + mat_a : g.w.y[g.cur ^ 1] + mat_y;
+                to += at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
+                swap_halves(hi_out);
+                *reinterpret_cast<u4*>(to) = hi_out;
+                if (HAS_LO) {
+                    swap_halves(lo_out);
+                    if (P == 3) *reinterpret_cast<u4*>(to + kLo) = lo_out;
+                    else *reinterpret_cast<u4*>(g.w.y_lo + mat_y + at<1>(j, g.w.ldm, ib + 16 * t) + 8 * half) = lo_out;
                 }
             }
+        }
+        }
+        if (MODE == kLast) {
+            // rows of 32 values of the result, two a wavefront and instruction, eight in flight
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const OutArgs& o = g.out;
+            const int ib0 = i0 + wi;
+#pragma unroll 1
+            for (int b = 0; b < 2 * F; b++) {
+                const int ib = ib0 + 32 * (b >> 1), p0 = 16 * (b & 1) + half;
+                const int row0 = (o.tall ? jb : ib) + p0, col = (o.tall ? ib : jb) + n32;
+                if (ib >= end_i) break;
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    v[k] = o.tall ? out_stage[b >> 1][n32][p0 + 2 * k] : out_stage[b >> 1][p0 + 2 * k][n32];
+                put_rows(o, bt * o.stride, row0, col, v);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
 }
 
 // steps = 0: the scaled input itself
@@ -395,50 +595,82 @@ __global__ __launch_bounds__(256) void k_ortho_copy(Work w, OutArgs t) {
         const int j = t.tall ? r : c, i = t.tall ? c : r;
         const _Float16* y = w.y[0] + bt * w.np * (size_t)w.ldm;
         const size_t o = at<P>(j, w.ldm, i);
-        const float v = (float)y[o] + (float)(P == 3 ? y[o + 32] : w.y_lo[(bt * w.np + j) * w.mp + i]);
+        const float v = (float)y[o] + (float)(P == 3 ? y[o + kLo] : w.y_lo[bt * w.np * (size_t)w.ldm + o]);
         put_out(t, bt * t.stride + (size_t)r * t.ld + c, v * (1.0f / kScaleX));
     }
 }
 
 // ---- plan ------------------------------------------------------------------------------
 struct Plan {
-    int tile, mp, np, ldm, ldn;
+    int mp, np, ldm, ldn, groups;
     size_t part, x, y, y_lo, ab, total;   // bytes
 };
+constexpr int kOverhang = 256 - 64;
 size_t round_up(size_t v, size_t q) { return (v + q - 1) / q * q; }
-// Tiles of 128 where they fill the machine, of 64 where they would leave most of it idle.
 Plan make_plan(int batch, int rows, int cols, int products) {
     Plan p{};
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    const int64_t big = (int64_t)((m + 127) / 128) * ((n + 127) / 128) * batch;
-    p.tile = big >= 192 ? 128 : 64;
-    p.mp = (int)round_up(m, p.tile);
-    p.np = (int)round_up(n, p.tile);
+    p.mp = (int)round_up(m, 64);
+    p.np = (int)round_up(n, 64);
     const int planes = products == 3 ? 2 : 1;
     p.ldm = p.mp * planes;
     p.ldn = p.np * planes;
     const size_t h = sizeof(_Float16);
-    p.part = round_up((size_t)batch * kNormGroups * sizeof(double), 256);
-    p.x = round_up((size_t)batch * p.mp * p.ldn * h, 256);
-    p.y = round_up((size_t)batch * p.np * p.ldm * h, 256);
-    p.y_lo = products == 1 ? round_up((size_t)batch * p.np * p.mp * h, 256) : 0;
-    p.ab = round_up((size_t)batch * p.mp * p.ldm * h, 256);
+    // a wavefront of the first pass takes two or more pieces of 256 columns
+    const int64_t units = (int64_t)rows * ((cols + 255) / 256);
+    p.groups = (int)(units / 8 < 1 ? 1 : units / 8 > kMaxNormGroups ? kMaxNormGroups : units / 8);
+    p.part = round_up((size_t)batch * p.groups * sizeof(double), 256);
+    // A tile that hangs over the last row of a batch reads up to kOverhang rows behind it: into
+    // the next matrix or this slack.  What it reads there reaches only rows that are not stored.
+    p.x = round_up(((size_t)batch * p.mp + kOverhang) * p.ldn * h, 256);
+    p.y = round_up(((size_t)batch * p.np + kOverhang) * p.ldm * h, 256);
+    p.y_lo = products == 1 ? round_up((size_t)batch * p.np * p.ldm * h, 256) : 0;
+    p.ab = round_up(((size_t)batch * p.mp + kOverhang) * p.ldm * h, 256);
     p.total = p.part + p.x + 2 * p.y + p.y_lo + 2 * p.ab;
     return p;
 }
 
-template <int P, int MODE, int WM, int WN, int FM, int FN>
+template <int P, int MODE, int F, int SUB, int R>
 void run_mul(MulArgs g, int batch, hipStream_t st) {
-    constexpr int TM = 32 * WM * FM, TN = 32 * WN * FN;
-    g.tiles_i = g.w.mp / TM;
-    g.tiles_j = (MODE == kGram || MODE == kPoly ? g.w.mp : g.w.np) / TN;
-    const int tiles = MODE == kGram || MODE == kPoly ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * g.tiles_j;
-    hipLaunchKernelGGL((k_ortho_mul<P, MODE, WM, WN, FM, FN>), dim3(tiles, batch), dim3(64 * WM * WN), 0, st, g);
+    constexpr int T = 64 * F;
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    g.tiles_i = (g.w.mp + T - 1) / T;
+    const int tiles_j = (g.w.np + T - 1) / T;
+    const int tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
+    g.row_len = SYM ? g.tiles_i + 1 : g.tiles_i;
+    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
+    hipLaunchKernelGGL((k_ortho_mul<P, MODE, F, SUB, R>), dim3(tiles, batch), dim3(256), 0, st, g);
 }
+// Tile size of a product: rounds of 256 workgroups (one a CU) times what a tile costs relative to
+// a 64 x 64 one.  A tile twice as wide does four times the work in 2.1 times the time: it reads
+// half as much from L2 and LDS an operation.  Measured at 4096 x 4096, P = 1: B X on tiles of
+// 256 / 192 / 128: 138 / 152 / 151 us; X X^T (253 tiles of 192 fill the machine, 136 of 256 half of
+// it): 82 / 70 / 90 us.  At 1000 x 2731, P = 3: B X on 192 / 128 / 64: 41 / 26 / 29 us, X X^T on
+// 128 / 64: 40 / 19 us.
+int tile_for(bool sym, int rows, int cols, int batch) {
+    constexpr float cost[5] = {0.0f, 1.0f, 2.1f, 4.3f, 7.5f};
+    int best = 1;
+    float least = 0.0f;
+    for (int f = 1; f <= 4; f++) {
+        const int64_t ti = (rows + 64 * f - 1) / (64 * f), tj = (cols + 64 * f - 1) / (64 * f);
+        const int64_t tiles = (sym ? ti * (ti + 1) / 2 : ti * tj) * batch;
+        const float c = (float)((tiles + 255) / 256) * cost[f];
+        if (f == 1 || c < least) { least = c; best = f; }
+    }
+    return best;
+}
+// Ring buffers: three to four stages in flight where they fit into 160 KiB (with two, a stage of
+// small tiles is over before the copies of the next have landed: 42 instead of 19 us above); tiles
+// of 128 with P = 1 run faster as two workgroups a CU of two stages each.
 template <int P, int MODE>
-void run_mul(const MulArgs& g, int tile, int batch, hipStream_t st) {
-    if (tile == 128) run_mul<P, MODE, 2, 2, 2, 2>(g, batch, st);
-    else run_mul<P, MODE, 2, 2, 1, 1>(g, batch, st);
+void run_mul(const MulArgs& g, int batch, hipStream_t st) {
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    switch (tile_for(SYM, g.w.mp, SYM ? g.w.mp : g.w.np, batch)) {
+        case 4: run_mul<P, MODE, 4, P == 1 ? 1 : 2, P == 1 ? 4 : 2>(g, batch, st); break;
+        case 3: run_mul<P, MODE, 3, 2, 3>(g, batch, st); break;
+        case 2: run_mul<P, MODE, 2, 2, P == 1 ? 2 : 4>(g, batch, st); break;
+        default: run_mul<P, MODE, 1, 2, 4>(g, batch, st); break;
+    }
 }
 
 template <int P>
@@ -447,6 +679,10 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
     Work w{};
     InArgs a = in;
     a.part = (double*)work;             work += p.part;
+    a.groups = p.groups;
+    a.vec = a.ld % 4 == 0 && a.stride % 4 == 0 &&
+            (reinterpret_cast<uintptr_t>(a.g) & (a.dtype == CFP_F32 ? 15u : 7u)) == 0 &&
+            (reinterpret_cast<uintptr_t>(a.mom) & 15u) == 0;
     w.x = (_Float16*)work;              work += p.x;
     w.y[0] = (_Float16*)work;           work += p.y;
     w.y[1] = (_Float16*)work;           work += p.y;
@@ -455,7 +691,7 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
     w.b = (_Float16*)work;
     w.mp = p.mp; w.np = p.np; w.ldm = p.ldm; w.ldn = p.ldn;
     const int tall = out.tall;
-    hipLaunchKernelGGL(k_ortho_norm, dim3(kNormGroups, batch), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_ortho_norm, dim3(p.groups, batch), dim3(256), 0, st, a);
     const int rp = tall ? p.np : p.mp, cp = tall ? p.mp : p.np;
     hipLaunchKernelGGL(k_ortho_load<P>, dim3(cp / 64, rp / 64, batch), dim3(256), 0, st, a, w, tall);
     if (steps == 0) {
@@ -469,13 +705,13 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
         g.cur = s & 1;
         g.a = coef[3 * s]; g.b = coef[3 * s + 1]; g.c = coef[3 * s + 2];
         g.out = out;
-        g.l = g.r = w.x; g.ldl = g.ldr = p.ldn; g.l_batch = g.r_batch = xb; g.stages = p.ldn / 64;
-        run_mul<P, kGram>(g, p.tile, batch, st);
-        g.l = g.r = w.a; g.ldl = g.ldr = p.ldm; g.l_batch = g.r_batch = ab; g.stages = p.ldm / 64;
-        run_mul<P, kPoly>(g, p.tile, batch, st);
-        g.l = w.b; g.r = w.y[g.cur]; g.ldl = g.ldr = p.ldm; g.l_batch = ab; g.r_batch = yb; g.stages = p.ldm / 64;
-        if (s + 1 < steps) run_mul<P, kStep>(g, p.tile, batch, st);
-        else run_mul<P, kLast>(g, p.tile, batch, st);
+        g.l = g.r = w.x; g.ldl = g.ldr = p.ldn; g.l_batch = g.r_batch = xb; g.stages = p.ldn / 32;
+        run_mul<P, kGram>(g, batch, st);
+        g.l = g.r = w.a; g.ldl = g.ldr = p.ldm; g.l_batch = g.r_batch = ab; g.stages = p.ldm / 32;
+        run_mul<P, kPoly>(g, batch, st);
+        g.l = w.b; g.r = w.y[g.cur]; g.ldl = g.ldr = p.ldm; g.l_batch = ab; g.r_batch = yb; g.stages = p.ldm / 32;
+        if (s + 1 < steps) run_mul<P, kStep>(g, batch, st);
+        else run_mul<P, kLast>(g, batch, st);
     }
     CFP_HIP_TRY(hipGetLastError());
     return 0;
@@ -537,7 +773,7 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
     float c[3 * kMaxSteps];
     fill_coef(coefs, steps, c);
     InArgs in{};
-    in.g = d_g; in.dtype = dtype; in.ld = ld; in.stride = batch_stride; in.rows = rows; in.cols = cols; in.eps = eps;
+    in.g = d_g; in.dtype = dtype; in.ld = ld; in.stride = batch > 1 ? batch_stride : 0; in.rows = rows; in.cols = cols; in.eps = eps;
     OutArgs out{};
     out.out = d_out; out.dtype = dtype; out.ld = ld_out; out.stride = out_batch_stride;
     out.rows = rows; out.cols = cols; out.tall = rows > cols;
@@ -566,7 +802,7 @@ int muon_update(const MuonArgs& u, hipStream_t st) {
     float c[3 * kMaxSteps];
     fill_coef(u.coefs, u.steps, c);
     InArgs in{};
-    in.g = u.g; in.dtype = CFP_F32; in.ld = u.ld; in.stride = u.stride; in.rows = u.rows; in.cols = u.cols;
+    in.g = u.g; in.dtype = CFP_F32; in.ld = u.ld; in.stride = u.batch > 1 ? u.stride : 0; in.rows = u.rows; in.cols = u.cols;
     in.mom = u.mom; in.beta = u.beta; in.nesterov = u.nesterov; in.eps = u.eps;
     in.g_clear = u.clear_g ? u.g : nullptr;
     OutArgs out{};

@@ -127,12 +127,13 @@ def test_sizes_of_values(pkg, cuda):
     """Squares that would overflow or vanish in 32 bits, a norm below eps, zeros, NaN, infinity."""
     torch = _torch()
     base = gradient(cuda, 1, 48, 80, seed=2, size=1.0)
-    for size in (1e30, 1e-4, 1e-30):
+    for size in (1e30, 1e-4, 1e-30, 1e-38):
         g = base * size
         assert off(pkg.policy.orthogonalize(g, eps=0.0), reference(g, eps=0.0)) <= tolerance("f32", 3, g.shape)
     small = base * 1e-9                    # |G| of the order of eps: not yet normalised, still right
     assert off(pkg.policy.orthogonalize(small), reference(small)) <= tolerance("f32", 3, base.shape)
     assert pkg.policy.orthogonalize(torch.zeros(2, 30, 50, device=cuda)).eq(0).all()
+    assert pkg.policy.orthogonalize(torch.zeros(2, 30, 50, device=cuda), eps=0.0).eq(0).all()
     g = torch.cat([base, base])
     g[1, 5, 7] = float("nan")
     got = pkg.policy.orthogonalize(g)
