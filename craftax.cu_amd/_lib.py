@@ -105,6 +105,10 @@ PROTOTYPES = {
     "cfp_train_backward": (C.c_int, [vp, C.c_int, C.c_int, vp]),
     "cfp_train_zero_loss": (C.c_int, [vp]*2),
     "cfp_train_adam": (C.c_int, [vp]*2),
+    "cfp_muon_defaults": (C.c_int, [vp]),
+    "cfp_train_set_optimizer": (C.c_int, [vp, C.c_int, vp, vp]),
+    "cfp_train_optimizer": (C.c_int, [vp]),
+    "cfp_train_muon": (C.c_int, [vp]*2),
     "cfp_train_update": (C.c_int, [vp, C.c_int, vp]),
     "cfp_train_loss": (C.c_int, [vp, vp, vp]),
     "cfp_synth_classic_records": (C.c_int, [vp, C.c_int, C.c_uint64, C.c_uint64, vp]),
@@ -153,9 +157,15 @@ class PpoConfig(C.Structure):
                 ("bwd_win", C.c_int)]
 
 
+class MuonConfig(C.Structure):
+    """cfp_muon_config of include/cfp.h."""
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float),
+                ("nesterov", C.c_int), ("steps", C.c_int)]
+
+
 BUF = {name: i for i, name in enumerate(
     ["r_obs", "r_state", "r_act", "r_logprob", "r_value", "r_reward", "r_done", "adv",
-     "ret", "v_boot", "stats", "loss_acc", "grads", "adam_m", "adam_v", "lr", "ent", "step_ctr"])}
+     "ret", "v_boot", "stats", "loss_acc", "grads", "adam_m", "adam_v", "lr", "ent", "step_ctr", "muon_lr"])}
 
 
 class CfpError(RuntimeError):

@@ -81,9 +81,11 @@ int launch_adv_moments(const float* adv, size_t count, double* part, double* mom
 
 // Adam step on the flat arena (k_adam :10668): params, moments updated, grads zeroed,
 // and every weight mirror of the full-game policy rewritten from the new values in
-// the same pass.  step_ctr is read, not bumped.
+// the same pass.  step_ctr is read, not bumped.  matrices_done: W_enc and W_gru hold their new
+// values already (a Muon step); the rest of the arena is updated and all mirrors are written.
 int launch_adam(cfp_policy* p, float* grads, float* m, float* v, const uint64_t* step_ctr,
-                const float* lr, float beta1, float beta2, float eps, hipStream_t st);
+                const float* lr, float beta1, float beta2, float eps, hipStream_t st,
+                bool matrices_done = false);
 
 // dW_enc from the records (enc_grad.hip) with the fp32 rows of its 75-feature remainder made
 // ahead of time: the expansion depends on the records only, so the update asks for it at the

@@ -621,6 +621,7 @@ struct AdamArgs {
     float* wg_pk; __bf16* wg_bf;
     float* wav_pk; __bf16* wav_bf;
     int layers;
+    int matrices_done;   // W_enc and W_gru were updated elsewhere: only their mirrors are written
     int enc_items, mid_items, tail_items;   // lanes of the three ranges below
     int off_b_enc, off_w_gru, off_w_a, off_b_a, off_w_v, off_b_v;
 };
@@ -677,7 +678,7 @@ __global__ __launch_bounds__(256) void k_adam_mirrors(AdamArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int f = 4 * fq + j;
-            w[j] = f < CFP_OBS ? adam_one(a, k, (size_t)f * H + u) : 0.0f;
+            w[j] = f >= CFP_OBS ? 0.0f : a.matrices_done ? a.params[(size_t)f * H + u] : adam_one(a, k, (size_t)f * H + u);
         }
         {   // fp32 mirror: K block fq / 2, lane half fq % 2
             const int kb = fq >> 1, lane = (fq & 1) * 32 + l32;
@@ -705,7 +706,8 @@ __global__ __launch_bounds__(256) void k_adam_mirrors(AdamArgs a) {
     if (it < a.mid_items) {
         // [b_enc | W_gru | W_a]: four consecutive floats of the arena
         const int o = a.off_b_enc + 4 * it;
-        const f4 w = adam_four(a, k, (size_t)o);
+        const f4 w = a.matrices_done && o >= a.off_w_gru && o < a.off_w_a
+                         ? *reinterpret_cast<const f4*>(a.params + o) : adam_four(a, k, (size_t)o);
         if (o < a.off_w_gru) return;   // b_enc is read from the arena
         if (o < a.off_w_a) {
             const int i = o - a.off_w_gru;
@@ -830,7 +832,7 @@ int launch_adv_moments(const float* adv, size_t count, double* part, double* mom
 }
 
 int launch_adam(cfp_policy* p, float* grads, float* m, float* v, const uint64_t* step_ctr,
-                const float* lr, float beta1, float beta2, float eps, hipStream_t st) {
+                const float* lr, float beta1, float beta2, float eps, hipStream_t st, bool matrices_done) {
     CFP_REQUIRE(p && p->variant == 0, "Adam with mirrors covers the full-game policy");
     const int L = p->layers;
     AdamArgs a{};
@@ -842,6 +844,7 @@ int launch_adam(cfp_policy* p, float* grads, float* m, float* v, const uint64_t*
     a.wg_pk = p->wg_pk; a.wg_bf = reinterpret_cast<__bf16*>(p->wg_bf);
     a.wav_pk = p->wav_pk; a.wav_bf = reinterpret_cast<__bf16*>(p->wav_bf);
     a.layers = L;
+    a.matrices_done = matrices_done ? 1 : 0;
     a.off_b_enc = CFP_OFF_B_ENC; a.off_w_gru = CFP_OFF_W_GRU; a.off_w_a = CFP_OFF_W_A(L);
     a.off_b_a = CFP_OFF_B_A(L); a.off_w_v = CFP_OFF_W_V(L); a.off_b_v = CFP_OFF_B_V(L);
     static_assert(CFP_OFF_B_ENC % 4 == 0 && CFP_OFF_W_GRU % 4 == 0 && (CFP_GRU * CFP_HIDDEN) % 4 == 0 &&

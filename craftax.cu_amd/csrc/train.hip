@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) void k_colsum_fold(const float* __restrict__ p
 }
 
 __global__ void k_bump_ctr(uint64_t* ctr) { *ctr += 1; }
+__global__ void k_zero_ctr(uint64_t* ctr) { *ctr = 0; }
 
 __global__ void k_take_value(const float* __restrict__ av, float* __restrict__ value_row,
                              int n) {
@@ -172,7 +173,7 @@ struct cfp_trainer {
     // the process-wide GEMM modes it was captured under
     hipGraph_t tgraph = nullptr;
     hipGraphExec_t texec = nullptr;
-    int graph_split = -1, graph_bf16 = -1, graph_pol_bf16 = -1, graph_store16 = -1;
+    int graph_split = -1, graph_bf16 = -1, graph_pol_bf16 = -1, graph_store16 = -1, graph_opt = -1;
     // bf16 storage of the window's gate pre-activations / their gradients and of the
     // layer inputs (in effect with bf16 GEMM inputs on the split kernels only)
     int bf16_store = 0;
@@ -183,6 +184,12 @@ struct cfp_trainer {
     double prof_ms[4] = {0.0, 0.0, 0.0, 0.0};   // rollout, gae (+ bootstrap), backward, adam
     // GEMM mode of this trainer's update (cfp_train_set_gemm_mode); -1: the process-wide switch
     int gemm_bf16 = -1, gemm_split = -1;
+    // optimiser of cfp_train_update (cfp_train_set_optimizer); opt_version counts its changes
+    int optimizer = CFP_OPT_ADAM, opt_version = 0;
+    cfp_muon_config muon{};
+    float* d_muon_lr = nullptr;
+    void *muon_gates = nullptr, *muon_enc = nullptr;   // workspaces, made by the first CFP_OPT_MUON
+    size_t muon_gates_bytes = 0, muon_enc_bytes = 0;
     hipStream_t st_own = nullptr;   // capture stream when the caller passes the null stream
 };
 
@@ -273,6 +280,7 @@ int cfp_train_create(cfp_trainer** out, cfp_policy* p, int T, const cfp_ppo_conf
     TA(boot_state, (size_t)tr->L * hn * sizeof(float));
     TA(d_lr, sizeof(float));
     TA(d_ent, sizeof(float));
+    TA(d_muon_lr, sizeof(float));
     TA(xobs, cc * kObsPad * sizeof(float));   // rows widened 843 -> 848: 16-byte aligned
     for (int l = 0; l <= tr->L; l++) TA(x[l], cc * H * sizeof(float));
     for (int l = 0; l < tr->L; l++) TA(preb[l], cc * G * sizeof(float));
@@ -333,6 +341,7 @@ void* cfp_train_buffer(cfp_trainer* tr, int which) {
         case CFP_BUF_LR: return tr->d_lr;
         case CFP_BUF_ENT: return tr->d_ent;
         case CFP_BUF_STEP_CTR: return tr->step_ctr;
+        case CFP_BUF_MUON_LR: return tr->d_muon_lr;
         default: return nullptr;
     }
 }
@@ -759,6 +768,101 @@ int cfp_train_adam(cfp_trainer* tr, void* stream) {
     return 0;
 }
 
+int cfp_muon_defaults(cfp_muon_config* cfg) {
+    CFP_REQUIRE(cfg, "cfp_muon_defaults: NULL");
+    cfg->lr = 0.02f; cfg->momentum = 0.95f; cfg->weight_decay = 0.0f;
+    cfg->nesterov = 1; cfg->steps = 5;
+    return 0;
+}
+
+int cfp_train_set_optimizer(cfp_trainer* tr, int kind, const cfp_muon_config* cfg, void* stream) {
+    CFP_REQUIRE(tr, "cfp_train_set_optimizer: NULL trainer");
+    CFP_REQUIRE(kind == CFP_OPT_ADAM || kind == CFP_OPT_MUON, "cfp_train_set_optimizer: kind must be CFP_OPT_ADAM or CFP_OPT_MUON (got %d)",
+                kind);
+    hipStream_t st = (hipStream_t)stream;
+    if (kind == CFP_OPT_MUON) {
+        cfp_muon_config c;
+        if (cfg) c = *cfg;
+        else cfp_muon_defaults(&c);
+        CFP_REQUIRE(c.steps >= 0 && c.steps <= 16 && c.momentum >= 0.0f && c.momentum < 1.0f,
+                    "cfp_train_set_optimizer: steps must be in 0..16 and momentum in [0, 1) (got %d, %g)", c.steps,
+                    (double)c.momentum);
+        if (!tr->muon_gates) {
+            // three products a product take more room than one: enough for either GEMM mode
+            size_t bytes[2] = {0, 0};
+            for (int p = 1; p <= 3; p += 2) {
+                const size_t g = cfp_orthogonalize_workspace(3 * tr->L, H, H, p), e = cfp_orthogonalize_workspace(1, CFP_OBS, H, p);
+                if (g > bytes[0]) bytes[0] = g;
+                if (e > bytes[1]) bytes[1] = e;
+            }
+            void* q[2] = {nullptr, nullptr};
+            CFP_HIP_TRY(hipMalloc(&q[0], bytes[0]));
+            const hipError_t e = hipMalloc(&q[1], bytes[1]);
+            if (e != hipSuccess) {
+                (void)hipFree(q[0]);
+                CFP_HIP_TRY(e);
+            }
+            tr->owned.push_back(q[0]);
+            tr->owned.push_back(q[1]);
+            tr->muon_gates = q[0]; tr->muon_gates_bytes = bytes[0];
+            tr->muon_enc = q[1]; tr->muon_enc_bytes = bytes[1];
+        }
+        tr->muon = c;
+        hipLaunchKernelGGL(k_fill, dim3(1), dim3(256), 0, st, tr->d_muon_lr, (size_t)1, c.lr);
+    }
+    if (kind != tr->optimizer) {
+        // the two keep different things in the moments
+        const size_t pc = tr->p->param_count;
+        hipLaunchKernelGGL(k_fill, dim3(grid1(pc)), dim3(256), 0, st, tr->adam_m, pc, 0.0f);
+        hipLaunchKernelGGL(k_fill, dim3(grid1(pc)), dim3(256), 0, st, tr->adam_v, pc, 0.0f);
+        hipLaunchKernelGGL(k_zero_ctr, dim3(1), dim3(1), 0, st, tr->adam_ctr);
+    }
+    tr->optimizer = kind;
+    tr->opt_version++;
+    CFP_HIP_TRY(hipGetLastError());
+    return 0;
+}
+int cfp_train_optimizer(const cfp_trainer* tr) { return tr ? tr->optimizer : -1; }
+
+int cfp_train_muon(cfp_trainer* tr, void* stream) {
+    CFP_REQUIRE(tr, "cfp_train_muon: NULL trainer");
+    CFP_REQUIRE(tr->optimizer == CFP_OPT_MUON, "cfp_train_muon: the trainer's optimiser is Adam (cfp_train_set_optimizer)");
+    hipStream_t st = (hipStream_t)stream;
+    cfp_policy* p = tr->p;
+    int bf = 0, split = 0;
+    if (cfp_train_gemm_mode(tr, &bf, &split)) return 1;
+    MuonArgs u{};
+    u.lr_dev = tr->d_muon_lr; u.lr = 1.0f;
+    u.beta = tr->muon.momentum; u.nesterov = tr->muon.nesterov; u.decay = tr->muon.weight_decay;
+    u.scale = 1.0f;   // no matrix here has more outputs than inputs: the gate blocks are square,
+                      // W_enc is stored [features][units]
+    u.steps = tr->muon.steps; u.eps = 1e-7f;
+    u.products = bf ? 1 : 3;   // bf16 GEMM inputs: one product here as well
+    u.clear_g = 1;
+    // W_enc on the second stream, the gate blocks [zh | zg | zp] of every layer beside it: both are
+    // chains of small launches that leave most CUs idle
+    CFP_HIP_TRY(hipEventRecord(tr->ev_head, st));
+    CFP_HIP_TRY(hipStreamWaitEvent(tr->st2, tr->ev_head, 0));
+    MuonArgs e = u;
+    e.w = p->params + CFP_OFF_W_ENC; e.g = tr->grads + CFP_OFF_W_ENC; e.mom = tr->adam_m + CFP_OFF_W_ENC;
+    e.ld = H; e.batch = 1; e.rows = CFP_OBS; e.cols = H;
+    e.work = tr->muon_enc; e.work_bytes = tr->muon_enc_bytes;
+    int rc = muon_update(e, tr->st2);
+    u.w = p->params + CFP_OFF_W_GRU; u.g = tr->grads + CFP_OFF_W_GRU; u.mom = tr->adam_m + CFP_OFF_W_GRU;
+    u.ld = H; u.stride = (int64_t)H * H; u.batch = 3 * tr->L; u.rows = u.cols = H;
+    u.work = tr->muon_gates; u.work_bytes = tr->muon_gates_bytes;
+    if (rc == 0) rc = muon_update(u, st);
+    // joined also after a failure: a capture must not end with the second stream still in it
+    CFP_HIP_TRY(hipEventRecord(tr->ev_join, tr->st2));
+    CFP_HIP_TRY(hipStreamWaitEvent(st, tr->ev_join, 0));
+    if (rc) return rc;
+    // biases and heads by Adam, and every weight mirror from the new values
+    if (launch_adam(p, tr->grads, tr->adam_m, tr->adam_v, tr->adam_ctr, tr->d_lr, 0.9f, 0.999f, 1e-8f, st, true)) return 1;
+    hipLaunchKernelGGL(k_bump_ctr, dim3(1), dim3(1), 0, st, tr->adam_ctr);
+    CFP_HIP_TRY(hipGetLastError());
+    return 0;
+}
+
 // cu_train_body without its collect (craftax_full.cu:13348-13366): per epoch the loss
 // sums start at zero, then every minibatch's backward is followed by its Adam step.
 static int train_body(cfp_trainer* tr, void* stream) {
@@ -768,7 +872,7 @@ static int train_body(cfp_trainer* tr, void* stream) {
             const double t0 = prof_mark(tr, stream);
             rc = cfp_train_backward(tr, m * tr->mb, tr->mb, stream);
             const double t1 = prof_mark(tr, stream);
-            if (rc == 0) rc = cfp_train_adam(tr, stream);
+            if (rc == 0) rc = tr->optimizer == CFP_OPT_MUON ? cfp_train_muon(tr, stream) : cfp_train_adam(tr, stream);
             prof_add(tr, 2, t0, t1);
             prof_add(tr, 3, t1, prof_mark(tr, stream));
         }
@@ -794,7 +898,8 @@ int cfp_train_update(cfp_trainer* tr, int use_graph, void* stream) {
               bf = tr->gemm_bf16 >= 0 ? tr->gemm_bf16 : cfp_get_gemm_bf16(),
               pbf = cfp_policy_gemm_bf16(tr->p);
     if (tr->texec && (split != tr->graph_split || bf != tr->graph_bf16 ||
-                      pbf != tr->graph_pol_bf16 || tr->bf16_store + 2 * tr->rs16 != tr->graph_store16)) {
+                      pbf != tr->graph_pol_bf16 || tr->bf16_store + 2 * tr->rs16 != tr->graph_store16 ||
+                      tr->opt_version != tr->graph_opt)) {
         (void)hipGraphExecDestroy(tr->texec);
         (void)hipGraphDestroy(tr->tgraph);
         tr->texec = nullptr;
@@ -826,6 +931,7 @@ int cfp_train_update(cfp_trainer* tr, int use_graph, void* stream) {
         tr->graph_bf16 = bf;
         tr->graph_pol_bf16 = pbf;
         tr->graph_store16 = tr->bf16_store + 2 * tr->rs16;
+        tr->graph_opt = tr->opt_version;
     }
     CFP_HIP_TRY(hipGraphLaunch(tr->texec, st));
     CFP_HIP_TRY(hipStreamSynchronize(st));

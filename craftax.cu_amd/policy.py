@@ -248,7 +248,7 @@ class Trainer:
             "grads": ((self.policy.param_count,), "<f4"),
             "adam_m": ((self.policy.param_count,), "<f4"),
             "adam_v": ((self.policy.param_count,), "<f4"), "lr": ((1,), "<f4"),
-            "ent": ((1,), "<f4"), "step_ctr": ((1,), "<i8"),
+            "ent": ((1,), "<f4"), "step_ctr": ((1,), "<i8"), "muon_lr": ((1,), "<f4"),
         }
         shape, ts = shapes[name]
         return _wrap(lib().cfp_train_buffer(self._h, _lib.BUF[name]), shape, ts)
@@ -309,6 +309,26 @@ class Trainer:
 
     def adam(self):
         _check(lib().cfp_train_adam(self._h, _stream()))
+
+    def set_optimizer(self, kind, **muon):
+        """"adam" or "muon" for update()'s steps (cfp_train_set_optimizer); muon: fields of
+        cfp_muon_config that differ from the defaults."""
+        cfg = _lib.MuonConfig()
+        _check(lib().cfp_muon_defaults(C.byref(cfg)))
+        for k, v in muon.items():
+            assert hasattr(cfg, k), k
+            setattr(cfg, k, v)
+        kinds = {"adam": 0, "muon": 1}
+        _need(kind in kinds, 'optimizer: "adam" or "muon"')
+        _check(lib().cfp_train_set_optimizer(self._h, kinds[kind], C.byref(cfg), _stream()))
+
+    @property
+    def optimizer(self):
+        return ("adam", "muon")[lib().cfp_train_optimizer(self._h)]
+
+    def muon(self):
+        """The optimiser step of a trainer set to "muon" (cfp_train_muon)."""
+        _check(lib().cfp_train_muon(self._h, _stream()))
 
     def update(self, use_graph=False):
         """cu_train_update (craftax_full.cu:13372) over the stored rollout."""

@@ -506,7 +506,8 @@ enum cfp_train_buf {
     CFP_BUF_R_VALUE, CFP_BUF_R_REWARD, CFP_BUF_R_DONE, CFP_BUF_ADV, CFP_BUF_RET,
     CFP_BUF_V_BOOT, CFP_BUF_STATS /* double[2] */, CFP_BUF_LOSS_ACC /* double[3] */,
     CFP_BUF_GRADS, CFP_BUF_ADAM_M, CFP_BUF_ADAM_V, CFP_BUF_LR /* float */,
-    CFP_BUF_ENT /* float */, CFP_BUF_STEP_CTR /* uint64: rollout steps taken */
+    CFP_BUF_ENT /* float */, CFP_BUF_STEP_CTR /* uint64: rollout steps taken */,
+    CFP_BUF_MUON_LR /* float */
 };
 /* Borrowed device pointer to one of the trainer's buffers (NULL if unknown). */
 void* cfp_train_buffer(cfp_trainer* tr, int which);
@@ -597,6 +598,27 @@ int cfp_train_zero_loss(cfp_trainer* tr, void* stream);
 /* cu_train_adam (craftax_full.cu:13337): Adam step from the grads arena (which
  * it zeroes), bumps the step counter, rebuilds the weight mirrors. */
 int cfp_train_adam(cfp_trainer* tr, void* stream);
+/* The optimiser of cfp_train_update's steps: CFP_OPT_ADAM (the default, the reference's) or
+ * CFP_OPT_MUON (no counterpart in the reference): the weight matrices -- W_enc and, of every
+ * layer, the three 256 x 256 gate blocks -- take a Muon step (cfp_muon_update with scale 1, momentum
+ * in the CFP_BUF_ADAM_M arena), biases and heads an Adam step with CFP_BUF_LR.  Muon's own lr
+ * lives in device memory (CFP_BUF_MUON_LR).  With bf16 GEMM inputs (this trainer's mode) its
+ * products are single as well, with fp32 inputs threefold.  cfg NULL = cfp_muon_defaults (lr
+ * 0.02, momentum 0.95, no decay, nesterov, 5 steps); it is not used for CFP_OPT_ADAM.  A change of
+ * kind zeroes both moment arenas and Adam's step counter (on `stream`); the first CFP_OPT_MUON
+ * allocates the workspaces.  The next cfp_train_update captures its graph again. */
+enum cfp_optimizer { CFP_OPT_ADAM = 0, CFP_OPT_MUON = 1 };
+typedef struct cfp_muon_config {
+    float lr, momentum, weight_decay;
+    int nesterov;
+    int steps;          /* Newton-Schulz steps, 0..16 */
+} cfp_muon_config;
+int cfp_muon_defaults(cfp_muon_config* cfg);
+int cfp_train_set_optimizer(cfp_trainer* tr, int kind, const cfp_muon_config* cfg, void* stream);
+int cfp_train_optimizer(const cfp_trainer* tr);
+/* One such step from the grads arena (which it zeroes); the trainer's optimiser must be
+ * CFP_OPT_MUON.  The counterpart of cfp_train_adam. */
+int cfp_train_muon(cfp_trainer* tr, void* stream);
 /* cu_train_body without its collect + cu_train_update (craftax_full.cu:13348-13406):
  * one PPO iteration over the stored rollout (slabs, adv/ret and the advantage
  * statistics already in place): epochs x (loss sums reset, minibatches x

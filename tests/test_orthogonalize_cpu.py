@@ -68,3 +68,12 @@ def test_python_checks_before_the_library(pkg):
         pkg.policy.orthogonalize(torch.zeros(4, 4))
     with pytest.raises(ValueError, match="w:"):
         pkg.policy.muon_update(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 4), 0.1)
+
+
+def test_optimizer_refusals(pkg):
+    lib = pkg.lib()
+    cfg = pkg._lib.MuonConfig()
+    assert lib.cfp_muon_defaults(C.byref(cfg)) == 0 and cfg.steps == 5 and cfg.nesterov == 1
+    assert lib.cfp_muon_defaults(None) != 0
+    assert lib.cfp_train_set_optimizer(None, 1, None, None) != 0 and b"NULL" in lib.cfp_last_error()
+    assert lib.cfp_train_muon(None, None) != 0 and lib.cfp_train_optimizer(None) == -1
