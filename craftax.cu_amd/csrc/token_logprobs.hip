@@ -77,54 +77,144 @@ __device__ __forceinline__ void join(Sums& a, float m, float s, float u) {
     a.s += b.s;
     a.u += b.u;
 }
-// all-reduce over `width` consecutive lanes (a power of two)
-template <int WIDTH>
-__device__ __forceinline__ void join_lanes(Sums& a) {
-    float top = a.m;
-#pragma unroll
-    for (int d = WIDTH / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, WIDTH));
-    raise_max(a, top);
-#pragma unroll
-    for (int d = WIDTH / 2; d > 0; d >>= 1) {
-        a.s += __shfl_xor(a.s, d, WIDTH);
-        a.u += __shfl_xor(a.u, d, WIDTH);
+// All-reduce over 16 or 64 consecutive lanes in a tree of fixed shape.  Rotations inside rows of
+// 16 lanes ride on the addition itself (a shuffle through LDS a step instead: 27 us for 262 144
+// rows of 43 where this takes XXX).
+template <int N>
+__device__ __forceinline__ float row_rotate(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + N, 0xf, 0xf, true));
+}
+template <int WIDTH, class Op>
+__device__ __forceinline__ float reduce_lanes(float v, Op op) {
+    static_assert(WIDTH == 16 || WIDTH == 64, "rows of 16 lanes or the wavefront");
+    v = op(v, row_rotate<8>(v));
+    v = op(v, row_rotate<4>(v));
+    v = op(v, row_rotate<2>(v));
+    v = op(v, row_rotate<1>(v));
+    if (WIDTH == 64) {
+        v = op(v, __shfl_xor(v, 16));
+        v = op(v, __shfl_xor(v, 32));
     }
+    return v;
+}
+template <int WIDTH>
+__device__ __forceinline__ float sum_lanes(float v) {
+    return reduce_lanes<WIDTH>(v, [](float a, float b) { return a + b; });
+}
+template <int WIDTH>
+__device__ __forceinline__ float max_lanes(float v) {
+    return reduce_lanes<WIDTH>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ void join_lanes(Sums& a) {
+    raise_max(a, max_lanes<64>(a.m));
+    a.s = sum_lanes<64>(a.s);
+    a.u = sum_lanes<64>(a.u);
 }
 
 // ---- the best `top` entries seen by one wavefront -----------------------------------
-// Lane i holds the entry of rank i (value, index), best first; -1 marks a free place.  Order:
-// larger value, then lower index.
+// Lane i holds the entry of rank i (value, index), best first; index -1 marks a free place.
+// Order: larger value, then lower index.  An entry that beats the one of rank top - 1 goes to a
+// buffer in LDS; when that holds 64, they are sorted across the lanes (21 exchanges) and merged
+// with the list (6).  On values in random order the bar rises fast enough for the merges to
+// number about log4(entries / 64); one insertion at a time, about top * ln(entries / top) of
+// them and each as long as a few exchanges, took 34 us for 1 x 131 072 where this takes XXX.
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
+template <int D>
+__device__ __forceinline__ unsigned xor_lane(unsigned v) {
+    if (D == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);
+    if (D == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);
+    if (D == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);
+    if (D < 32) return __builtin_amdgcn_ds_swizzle(v, (D << 10) | 0x1f);
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+}
+struct Entry {
+    float v;
+    int i;
+};
+// keeps the better of this lane's and lane ^ D's entry where `better`, else the worse
+template <int D>
+__device__ __forceinline__ void exchange(Entry& e, bool better) {
+    const float ov = __uint_as_float(xor_lane<D>(__float_as_uint(e.v)));
+    const int oi = (int)xor_lane<D>((unsigned)e.i);
+    if (before(ov, oi, e.v, e.i) == better) { e.v = ov; e.i = oi; }
+}
+// runs of 2 D become sorted, alternately best first and last (by bit 2 D of the lane), from runs
+// of D that alternate
+template <int D, int STEP = D>
+__device__ __forceinline__ void merge_runs(Entry& e, bool best_first) {
+    const bool low = (threadIdx.x & STEP) == 0;
+    exchange<STEP>(e, low == best_first);
+    if constexpr (STEP > 1) merge_runs<D, STEP / 2>(e, best_first);
+}
+constexpr int kBuffer = 128;   // of which 64 trigger a merge
 struct Best {
-    float v = -INFINITY;
-    int i = -1;
+    Entry e{-INFINITY, -1};
     float last_v = -INFINITY;   // the entry of rank top - 1: what a newcomer has to beat
     int last_i = -1;
-    // wave-uniform (nv, ni)
-    __device__ __forceinline__ void insert(float nv, int ni, int top) {
-        const int lane = (int)(threadIdx.x & 63);
-        const int pos = __popcll(__ballot(before(v, i, nv, ni)));
-        const float pv = __shfl_up(v, 1);
-        const int pi = __shfl_up(i, 1);
-        if (lane > pos) { v = pv; i = pi; }
-        if (lane == pos) { v = nv; i = ni; }
-        last_v = lane_value(v, top - 1);
-        last_i = __builtin_amdgcn_readlane(i, top - 1);
+    int waiting = 0;            // entries in the buffer; wave-uniform
+    float2* buffer;             // [kBuffer] of this wavefront
+
+    // A bar for an empty list: every lane names the largest of the entries that it is about to
+    // offer, and what does not reach the top-th largest of those cannot be among the best.  Of a
+    // first tile about 1.2 top entries remain.
+    __device__ __forceinline__ void set_bar(float largest, int top) {
+        if (last_v != -INFINITY) return;
+        Entry c{largest, (int)(threadIdx.x & 63)};
+        sort(c, true);
+        last_v = lane_value(c.v, top - 1);
+        last_i = last_v == -INFINITY ? -1 : 0x7fffffff;   // entries equal to the bar pass
+    }
+    __device__ __forceinline__ static void sort(Entry& c, bool best_first) {
+        const int lane = threadIdx.x & 63;
+        merge_runs<1>(c, (lane & 2) == 0);
+        merge_runs<2>(c, (lane & 4) == 0);
+        merge_runs<4>(c, (lane & 8) == 0);
+        merge_runs<8>(c, (lane & 16) == 0);
+        merge_runs<16>(c, (lane & 32) == 0);
+        merge_runs<32>(c, best_first);
+    }
+    // the first 64 of the buffer into the list
+    __device__ __forceinline__ void merge(int top) {
+        const int lane = threadIdx.x & 63;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        Entry c{-INFINITY, -1};
+        if (lane < waiting) {
+            const float2 q = buffer[lane];
+            c = Entry{q.x, __float_as_int(q.y)};
+        }
+        if (waiting > 64) {   // the rest moves to the front
+            const float2 q = buffer[64 + lane];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            buffer[lane] = q;
+        }
+        waiting = waiting > 64 ? waiting - 64 : 0;
+        sort(c, false);   // worst first: against the list it makes one bitonic run
+        if (before(c.v, c.i, e.v, e.i)) e = c;
+        merge_runs<32>(e, true);
+        last_v = lane_value(e.v, top - 1);
+        last_i = __builtin_amdgcn_readlane(e.i, top - 1);
     }
     // one entry a lane (wave-uniform call); entries of -inf and NaN never enter: the free
     // places compare as (-inf, -1), which nothing of value -inf comes before
     __device__ __forceinline__ void offer(float x, int idx, int top) {
-        unsigned long long todo = __ballot(before(x, idx, last_v, last_i));
-        while (todo) {
-            const int l = __ffsll(todo) - 1;
-            todo &= todo - 1;
-            const float nv = lane_value(x, l);
-            const int ni = __builtin_amdgcn_readlane(idx, l);
-            if (before(nv, ni, last_v, last_i)) insert(nv, ni, top);
+        const bool mine = before(x, idx, last_v, last_i);
+        const unsigned long long who = __ballot(mine);
+        if (who == 0) return;
+        if (mine) {
+            const int at = waiting + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+            buffer[at] = make_float2(x, __int_as_float(idx));
         }
+        waiting += __popcll(who);
+        if (waiting >= 64) merge(top);
+    }
+    __device__ __forceinline__ void finish(int top) {
+        if (waiting > 0) merge(top);
     }
 };
 
@@ -178,12 +268,11 @@ __device__ __forceinline__ float token_logit(const LpArgs& a, int row, int tok) 
     return x;
 }
 
-// ---- short rows: L lanes a row, up to four entries a lane -----------------------------
+// ---- short rows: L lanes a row, R <= 4 entries a lane ----------------------------------
 // Each load instruction of a lane group covers L consecutive entries of its row.  No online
 // rescaling: the row sits in registers.  kShortMax entries at most.
-constexpr int kShortR = 4;
-constexpr int kShortMax = 64 * kShortR;
-template <typename T, int L, bool MASK>
+constexpr int kShortMax = 64 * 4;
+template <typename T, int L, int R, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
@@ -195,30 +284,26 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
         const uint8_t* mask = MASK ? a.mask + (size_t)r * a.ld_mask : nullptr;
         const int tok = a.tok[r];
         const float xt = token_logit<T>(a, r, tok);
-        float v[kShortR];
+        float v[R];
         Sums z;
 #pragma unroll
-        for (int j = 0; j < kShortR; j++) {
+        for (int j = 0; j < R; j++) {
             const int i = j * L + sub;
             v[j] = -INFINITY;
             if (i < a.vocab && (!MASK || mask[i])) v[j] = to_f32(x[i]);
             z.m = fmaxf(z.m, v[j]);
         }
+        z.m = max_lanes<L>(z.m);
 #pragma unroll
-        for (int d = L / 2; d > 0; d >>= 1) z.m = fmaxf(z.m, __shfl_xor(z.m, d, L));
-#pragma unroll
-        for (int j = 0; j < kShortR; j++) add_entry(z, v[j]);
-#pragma unroll
-        for (int d = L / 2; d > 0; d >>= 1) {
-            z.s += __shfl_xor(z.s, d, L);
-            z.u += __shfl_xor(z.u, d, L);
-        }
+        for (int j = 0; j < R; j++) add_entry(z, v[j]);
+        z.s = sum_lanes<L>(z.s);
+        z.u = sum_lanes<L>(z.u);
         if (live && sub == 0) write_row(a, row, z, tok, xt);
         for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
             float bv = -INFINITY;
             int bi = -1;
 #pragma unroll
-            for (int j = 0; j < kShortR; j++)   // ascending index: ties keep the first
+            for (int j = 0; j < R; j++)   // ascending index: ties keep the first
                 if (v[j] > bv) { bv = v[j]; bi = j * L + sub; }
 #pragma unroll
             for (int d = L / 2; d > 0; d >>= 1) {
@@ -227,91 +312,193 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
                 if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
             }
 #pragma unroll
-            for (int j = 0; j < kShortR; j++)
+            for (int j = 0; j < R; j++)
                 if (j * L + sub == bi) v[j] = -INFINITY;
             if (live && sub == 0) write_top(a, row, z, k, bv, bi);
         }
     }
 }
 
-// ---- long rows -------------------------------------------------------------------------
-// One tile: U vectors a lane, all loads in flight before the first use.
-constexpr int kU = 4;
-template <typename T, bool MASK, bool TOP>
-__device__ __forceinline__ void take_tile(const float (&v)[kU][Vec<T>::N], int i0, int vec_stride, Sums& z,
-                                          Best& best, int top) {
-    constexpr int N = Vec<T>::N;
-    float tm = v[0][0];
-#pragma unroll
-    for (int q = 0; q < kU; q++)
-#pragma unroll
-        for (int j = 0; j < N; j++) tm = fmaxf(tm, v[q][j]);
-    if (tm > z.m) raise_max(z, tm);
-#pragma unroll
-    for (int q = 0; q < kU; q++)
-#pragma unroll
-        for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
-    if (TOP && __any(tm >= best.last_v && tm > -INFINITY)) {
-#pragma unroll
-        for (int q = 0; q < kU; q++)
-#pragma unroll
-            for (int j = 0; j < N; j++) best.offer(v[q][j], i0 + q * vec_stride + j, top);
+// ---- short rows, many of them: one thread a row ------------------------------------------
+// The lanes of the kernel above spend 37 instructions a row (reductions, addresses, logarithm, each
+// on all 16 lanes); with rows staged through LDS and one thread a row it is about 8, and the
+// kernel is bound by HBM.  Fewer rows leave the machine idle this way: from kRowsFrom on.
+// The rows of LDS are an odd number of floats apart, so the threads' rows start in different banks.
+// Rows travel as 16-byte vectors whatever their alignment; the last vector of a row is moved back
+// to end with it, so it overlaps the one before (whose entries it repeats).
+constexpr int kRowsMax = 64, kRowsThreads = 128, kRowsFrom = 16384;
+__host__ __device__ inline int rows_pitch(int vocab) { return vocab | 1; }
+// vector q of kRowsThreads rows of `vocab` entries: its row and first entry
+template <int N>
+struct RowVectors {
+    int vocab, per_row;
+    unsigned inv;
+    __device__ __forceinline__ explicit RowVectors(int v) : vocab(v), per_row((v + N - 1) / N) {
+        inv = ((1u << 20) + per_row - 1) / per_row;   // q / per_row = q * inv / 2^20 for q < 2^11
     }
+    __device__ __forceinline__ void at(int q, int& row, int& first) const {
+        row = (int)(((unsigned)q * inv) >> 20);
+        first = min((q - row * per_row) * N, vocab - N);
+    }
+};
+// Rows [r0, r0 + kRowsThreads) of x as fp32 into LDS, -inf where masked; all of a thread's loads in
+// flight together (at most PASSES; per_row of them).
+template <typename T, int PASSES, bool MASK>
+__device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t* mask, int64_t ld_mask, int r0, int rows,
+                                           int vocab, float* stage) {
+    constexpr int N = Vec<T>::N;
+    const RowVectors<N> rv(vocab);
+    Vec<T> v[PASSES];
+    uint8_t mk[PASSES][N];
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        int r, i;
+        rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
+        if (p >= rv.per_row || r0 + r >= rows) continue;
+        v[p] = load_vec(x + (size_t)(r0 + r) * ld + i);
+        if (MASK) __builtin_memcpy(mk[p], mask + (size_t)(r0 + r) * ld_mask + i, N);
+    }
+    const int pitch = rows_pitch(vocab);
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        int r, i;
+        rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
+        if (p >= rv.per_row || r0 + r >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < N; j++) stage[r * pitch + i + j] = MASK && mk[p][j] == 0 ? -INFINITY : to_f32(v[p].v[j]);
+    }
+}
+template <typename T, int PASSES, bool MASK>
+__global__ __launch_bounds__(kRowsThreads) void k_logprobs_rows(LpArgs a) {
+    extern __shared__ float stage[];
+    for (int r0 = (int)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int)gridDim.x * kRowsThreads) {
+        const int row = r0 + (int)threadIdx.x;
+        stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
+        const int tok = row < a.rows ? a.tok[row] : -1;
+        __syncthreads();
+        if (row < a.rows) {
+            const float* x = stage + threadIdx.x * rows_pitch(a.vocab);
+            Sums z;
+#pragma unroll 4
+            for (int i = 0; i < a.vocab; i++) z.m = fmaxf(z.m, x[i]);
+#pragma unroll 4
+            for (int i = 0; i < a.vocab; i++) add_entry(z, x[i]);
+            write_row(a, row, z, tok, tok >= 0 && tok < a.vocab ? x[tok] : -INFINITY);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- long rows -------------------------------------------------------------------------
+// One tile: kU vectors a lane, all loads in flight before the first use.
+constexpr int kU = 4;
+// Candidates of a tile: lanes that hold one put their 64 bytes of it into LDS (raw type, masked
+// entries as -inf), rows kLaneBytes apart, and the wavefront offers one or a few such lanes'
+// entries at a time.  (Offering the 32 registers in turn is 32 copies of the merge: 298 us for
+// 4096 x 131 072 instead of XXX.)
+constexpr int kLaneBytes = 80;
+struct TopSpace {
+    float2 buffer[kBuffer];
+    __align__(16) unsigned char tile[64 * kLaneBytes];
+};
+template <typename T>
+__device__ __forceinline__ void offer_tile(const float (&v)[kU][Vec<T>::N], float tm, int base, int stride, int lane0,
+                                           unsigned char* tile, Best& best, int top) {
+    constexpr int N = Vec<T>::N, PER = kU * N, TOGETHER = 64 / PER;
+    const int lane = threadIdx.x & 63;
+    best.set_bar(tm, top);
+    const bool mine = tm >= best.last_v && tm > -INFINITY;
+    unsigned long long todo = __ballot(mine);
+    if (todo == 0) return;
+    if (mine)
+#pragma unroll
+        for (int q = 0; q < kU; q++) {
+            Vec<T> raw;
+#pragma unroll
+            for (int j = 0; j < N; j++) raw.v[j] = (T)v[q][j];   // exact: it came from a T
+            *reinterpret_cast<u4*>(tile + lane * kLaneBytes + 16 * q) = __builtin_bit_cast(u4, raw);
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int slot = lane % PER, q = slot / N, j = slot % N;
+    while (todo) {
+        int src = -1;
+#pragma unroll
+        for (int k = 0; k < TOGETHER; k++) {
+            if (todo && lane / PER == k) src = __ffsll((long long)todo) - 1;
+            todo &= todo - 1;   // 0 stays 0
+        }
+        float x = -INFINITY;
+        int idx = 0;   // not below -1: (-inf, -2) would come before a free place
+        if (src >= 0) {
+            x = to_f32(*reinterpret_cast<const T*>(tile + src * kLaneBytes + 16 * q + j * (int)sizeof(T)));
+            idx = base + q * stride + (lane0 + src) * N + j;
+        }
+        best.offer(x, idx, top);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // W wavefronts of a workgroup stream entries [lo, hi) of a row; thread t takes vectors t,
 // t + 64 W, ...  Every wavefront runs the same number of tiles (uniform trip count).
 template <typename T, bool MASK, bool TOP, int W>
 __device__ __forceinline__ void stream_row(const T* x, const uint8_t* mask, int lo, int hi, Sums& z, Best& best,
-                                           int top) {
+                                           TopSpace* space, int top) {
     constexpr int N = Vec<T>::N, STRIDE = 64 * W * N, TILE = STRIDE * kU;
     const int t = W == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
-    int base = lo;
-    float v[kU][N];
-    for (; base + TILE <= hi; base += TILE) {
+    for (int base = lo; base < hi; base += TILE) {
         const int i0 = base + t * N;
-        Vec<T> raw[kU];
-        uint8_t mk[kU][N];
+        float v[kU][N];
+        if (base + TILE <= hi) {
+            Vec<T> raw[kU];
+            uint8_t mk[kU][N];
 #pragma unroll
-        for (int q = 0; q < kU; q++) {
-            raw[q] = load_vec(x + i0 + q * STRIDE);
-            if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
-        }
-#pragma unroll
-        for (int q = 0; q < kU; q++)
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                v[q][j] = to_f32(raw[q].v[j]);
-                if (MASK && mk[q][j] == 0) v[q][j] = -INFINITY;
+            for (int q = 0; q < kU; q++) {
+                raw[q] = load_vec(x + i0 + q * STRIDE);
+                if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
             }
-        take_tile<T, MASK, TOP>(v, i0, STRIDE, z, best, top);
-    }
-    if (base < hi) {   // the last, partial tile: whole vectors where they fit, entries at the end
-        const int i0 = base + t * N;
 #pragma unroll
-        for (int q = 0; q < kU; q++) {
-            const int i = i0 + q * STRIDE;
-            if (i + N <= hi) {
-                const Vec<T> raw = load_vec(x + i);
-                uint8_t mk[N];
-                if (MASK) __builtin_memcpy(mk, mask + i, N);
+            for (int q = 0; q < kU; q++)
 #pragma unroll
-                for (int j = 0; j < N; j++) v[q][j] = MASK && mk[j] == 0 ? -INFINITY : to_f32(raw.v[j]);
-            } else {
+                for (int j = 0; j < N; j++) v[q][j] = MASK && mk[q][j] == 0 ? -INFINITY : to_f32(raw[q].v[j]);
+        } else {   // the last, partial tile: whole vectors where they fit, entries at the end
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    v[q][j] = -INFINITY;
-                    if (i + j < hi && (!MASK || mask[i + j])) v[q][j] = to_f32(x[i + j]);
+            for (int q = 0; q < kU; q++) {
+                const int i = i0 + q * STRIDE;
+                if (i + N <= hi) {
+                    const Vec<T> raw = load_vec(x + i);
+                    uint8_t mk[N];
+                    if (MASK) __builtin_memcpy(mk, mask + i, N);
+#pragma unroll
+                    for (int j = 0; j < N; j++) v[q][j] = MASK && mk[j] == 0 ? -INFINITY : to_f32(raw.v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        v[q][j] = -INFINITY;
+                        if (i + j < hi && (!MASK || mask[i + j])) v[q][j] = to_f32(x[i + j]);
+                    }
                 }
             }
         }
-        take_tile<T, MASK, TOP>(v, i0, STRIDE, z, best, top);
+        float tm = v[0][0];
+#pragma unroll
+        for (int q = 0; q < kU; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) tm = fmaxf(tm, v[q][j]);
+        if (tm > z.m) raise_max(z, tm);
+#pragma unroll
+        for (int q = 0; q < kU; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
+        if (TOP) offer_tile<T>(v, tm, base, STRIDE, t - (int)(threadIdx.x & 63), space->tile, best, top);
     }
 }
 
 // One wavefront a row, four rows a workgroup: rows that are many or not long.
 template <typename T, bool MASK, bool TOP>
 __global__ __launch_bounds__(256) void k_logprobs_wave(LpArgs a) {
+    __shared__ TopSpace spaces[TOP ? 4 : 1];
     const int lane = threadIdx.x & 63;
     for (int row0 = (int)blockIdx.x * 4; row0 < a.rows; row0 += (int)gridDim.x * 4) {
         const int row = row0 + (int)(threadIdx.x >> 6);
@@ -320,11 +507,15 @@ __global__ __launch_bounds__(256) void k_logprobs_wave(LpArgs a) {
         const float xt = token_logit<T>(a, row, tok);
         Sums z;
         Best best;
+        TopSpace* space = &spaces[TOP ? threadIdx.x >> 6 : 0];
+        best.buffer = space->buffer;
         stream_row<T, MASK, TOP, 1>((const T*)a.x + (size_t)row * a.ld,
-                                    MASK ? a.mask + (size_t)row * a.ld_mask : nullptr, 0, a.vocab, z, best, a.top);
-        join_lanes<64>(z);
+                                    MASK ? a.mask + (size_t)row * a.ld_mask : nullptr, 0, a.vocab, z, best, space,
+                                    a.top);
+        join_lanes(z);
         if (lane == 0) write_row(a, row, z, tok, xt);
-        if (TOP && lane < a.top) write_top(a, row, z, lane, best.v, best.i);
+        if (TOP) best.finish(a.top);
+        if (TOP && lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
     }
 }
 
@@ -334,7 +525,8 @@ constexpr int kWaves = 4;
 template <typename T, bool MASK, bool TOP>
 __global__ __launch_bounds__(64 * kWaves) void k_logprobs_group(LpArgs a) {
     __shared__ float zs[kWaves][3];
-    __shared__ float2 lists[kWaves][kMaxTop];
+    __shared__ TopSpace spaces[TOP ? kWaves : 1];
+    __shared__ float2 lists[TOP ? kWaves : 1][kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
     const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
@@ -342,33 +534,39 @@ __global__ __launch_bounds__(64 * kWaves) void k_logprobs_group(LpArgs a) {
     const float xt = a.splits == 1 ? token_logit<T>(a, row, tok) : 0.0f;
     Sums z;
     Best best;
+    TopSpace* space = &spaces[TOP ? wave : 0];
+    best.buffer = space->buffer;
     stream_row<T, MASK, TOP, kWaves>((const T*)a.x + (size_t)row * a.ld,
-                                     MASK ? a.mask + (size_t)row * a.ld_mask : nullptr, lo, hi, z, best, a.top);
-    join_lanes<64>(z);
+                                     MASK ? a.mask + (size_t)row * a.ld_mask : nullptr, lo, hi, z, best, space, a.top);
+    join_lanes(z);
     if (lane == 0) { zs[wave][0] = z.m; zs[wave][1] = z.s; zs[wave][2] = z.u; }
-    if (TOP && wave > 0 && lane < a.top) lists[wave][lane] = make_float2(best.v, __int_as_float(best.i));
+    if (TOP) best.finish(a.top);
+    if (TOP && wave > 0 && lane < a.top) lists[wave][lane] = make_float2(best.e.v, __int_as_float(best.e.i));
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
     for (int w = 1; w < kWaves; w++) join(z, zs[w][0], zs[w][1], zs[w][2]);
-    if (TOP)
+    if (TOP) {
         for (int w = 1; w < kWaves; w++) {
             const float2 e = lane < a.top ? lists[w][lane] : make_float2(-INFINITY, __int_as_float(-1));
             best.offer(e.x, __float_as_int(e.y), a.top);
         }
+        best.finish(a.top);
+    }
     if (a.splits == 1) {
         if (lane == 0) write_row(a, row, z, tok, xt);
-        if (TOP && lane < a.top) write_top(a, row, z, lane, best.v, best.i);
+        if (TOP && lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
         return;
     }
     const size_t o = (size_t)row * a.splits + split;
     if (lane == 0) a.part[o] = f4{z.m, z.s, z.u, 0.0f};
-    if (TOP && lane < a.top) a.part_top[o * a.top + lane] = make_float2(best.v, __int_as_float(best.i));
+    if (TOP && lane < a.top) a.part_top[o * a.top + lane] = make_float2(best.e.v, __int_as_float(best.e.i));
 }
 
 // One wavefront a row: the parts of its splits in ascending order of lane, then the tree.
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs a) {
+    __shared__ float2 buffer[kBuffer];
     const int lane = threadIdx.x, row = (int)blockIdx.x;
     const int tok = a.tok[row];
     const float xt = token_logit<T>(a, row, tok);
@@ -377,17 +575,20 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs a) {
         const f4 p = a.part[(size_t)row * a.splits + s];
         join(z, p[0], p[1], p[2]);
     }
-    join_lanes<64>(z);
+    join_lanes(z);
     if (lane == 0) write_row(a, row, z, tok, xt);
     if (a.top > 0) {
         Best best;
+        best.buffer = buffer;
+        best.set_bar(lane < a.splits ? a.part_top[((size_t)row * a.splits + lane) * a.top].x : -INFINITY, a.top);
         const int total = a.splits * a.top;
         for (int o = 0; o < total; o += 64) {
             float2 e = make_float2(-INFINITY, __int_as_float(-1));
             if (o + lane < total) e = a.part_top[(size_t)row * total + o + lane];
             best.offer(e.x, __float_as_int(e.y), a.top);
         }
-        if (lane < a.top) write_top(a, row, z, lane, best.v, best.i);
+        best.finish(a.top);
+        if (lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
     }
 }
 
@@ -444,14 +645,7 @@ __device__ __forceinline__ void row_grad(const LpGradArgs& a, int row, float wei
     r.weight = weight;
     r.g_ent = a.g_ent ? a.g_ent[row] : 0.0f;
 }
-template <int WIDTH>
-__device__ __forceinline__ float sum_lanes(float v) {
-#pragma unroll
-    for (int d = WIDTH / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, WIDTH);
-    return v;
-}
-
-template <typename T, int L, bool MASK>
+template <typename T, int L, int R, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_grad_short(LpGradArgs a) {
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
@@ -461,33 +655,89 @@ __global__ __launch_bounds__(256) void k_logprobs_grad_short(LpGradArgs a) {
         const int r = live ? row : a.rows - 1;
         const T* x = (const T*)a.x + (size_t)r * a.ld;
         const uint8_t* mask = MASK ? a.mask + (size_t)r * a.ld_mask : nullptr;
-        float v[kShortR], d[kShortR];
-        float weight = 0.0f;
+        float v[R], d[R];
 #pragma unroll
-        for (int j = 0; j < kShortR; j++) {
+        for (int j = 0; j < R; j++) {
             const int i = j * L + sub;
             v[j] = -INFINITY;
             if (i < a.vocab && (!MASK || mask[i])) v[j] = to_f32(x[i]);
             d[j] = 0.0f;
         }
+        // the named entries: whose lane holds an allowed one takes its gradient
+        float weight = 0.0f;
         for (int j = 0; j <= a.top; j++) {
-            float g;
-            const int i = named_entry<T>(a, r, j, g);
-            weight += g;
+            if (j == 0 && !a.g_lp) continue;
+            const int i = j == 0 ? a.tok[r] : a.ids[(size_t)r * a.top + j - 1];
+            const float g = j == 0 ? a.g_lp[r] : a.g_top[(size_t)r * a.top + j - 1];
+            if (i >= a.vocab && sub == 0) weight = NAN;
 #pragma unroll
-            for (int q = 0; q < kShortR; q++)
-                if (q * L + sub == i) d[q] += g;
+            for (int q = 0; q < R; q++)
+                if (q * L + sub == i && !(v[q] == -INFINITY)) { d[q] += g; weight += g; }
         }
         RowGrad rg;
-        row_grad(a, r, weight, rg);
+        row_grad(a, r, sum_lanes<L>(weight), rg);
         T* dx = (T*)a.dx + (size_t)r * a.ld_dx;
 #pragma unroll
-        for (int j = 0; j < kShortR; j++) {
+        for (int j = 0; j < R; j++) {
             const int i = j * L + sub;
             const bool on = !rg.none && !(v[j] == -INFINITY);
             // every load of this row was used above: the row may be overwritten in place
             if (live && i < a.vocab) dx[i] = (T)(on ? rg.at(v[j]) + d[j] : 0.0f);
         }
+    }
+}
+
+// one thread a row, as k_logprobs_rows; the gradient replaces the logits in LDS
+template <typename T, int PASSES, bool MASK>
+__global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs a) {
+    extern __shared__ float stage[];
+    constexpr int N = Vec<T>::N;
+    const int pitch = rows_pitch(a.vocab);
+    for (int r0 = (int)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int)gridDim.x * kRowsThreads) {
+        const int row = r0 + (int)threadIdx.x;
+        stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
+        int tok = -1;
+        float g = 0.0f;
+        if (row < a.rows && a.g_lp) { tok = a.tok[row]; g = a.g_lp[row]; }
+        __syncthreads();
+        if (row < a.rows) {
+            float* x = stage + threadIdx.x * pitch;
+            const bool hit = tok >= 0 && tok < a.vocab && !(x[tok] == -INFINITY);
+            RowGrad rg;
+            row_grad(a, row, tok >= a.vocab ? NAN : hit ? g : 0.0f, rg);
+#pragma unroll 4
+            for (int i = 0; i < a.vocab; i++) {
+                const float v = x[i];
+                x[i] = rg.none || v == -INFINITY ? 0.0f : rg.at(v) + (i == tok ? g : 0.0f);
+            }
+        }
+        __syncthreads();
+        const int here = min(kRowsThreads, a.rows - r0) * pitch;
+        if (a.ld_dx == pitch && here % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
+            // rows without gaps, in LDS and in memory: one run of aligned vectors (r0 * pitch is a
+            // multiple of kRowsThreads)
+            T* dx = (T*)a.dx + (size_t)r0 * pitch;
+#pragma unroll 4
+            for (int e = (int)threadIdx.x * N; e < here; e += kRowsThreads * N) {
+                Vec<T> out;
+#pragma unroll
+                for (int j = 0; j < N; j++) out.v[j] = (T)stage[e + j];
+                store_vec(dx + e, out);
+            }
+        } else {
+            const RowVectors<N> rv(a.vocab);
+#pragma unroll
+            for (int p = 0; p < PASSES; p++) {
+                int r, i;
+                rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
+                if (p >= rv.per_row || r0 + r >= a.rows) continue;
+                Vec<T> out;
+#pragma unroll
+                for (int j = 0; j < N; j++) out.v[j] = (T)stage[r * pitch + i + j];
+                store_vec((T*)a.dx + (size_t)(r0 + r) * a.ld_dx + i, out);   // repeated entries: the same values
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -562,7 +812,7 @@ struct LpPlan {
 LpPlan plan_forward(int rows, int vocab) {
     if (vocab <= kShortMax) return {0, 1, 0};
     if (rows >= 4096 && vocab <= 8192) return {1, 1, 0};
-    const int want = rows >= 1024 ? 1 : (1024 + rows - 1) / rows;
+    const int want = rows >= 512 ? 1 : (1024 + rows - 1) / rows;
     const int most = (vocab + 4095) / 4096;
     int splits = want < most ? want : most;
     const int chunk = ((vocab + splits - 1) / splits + 7) / 8 * 8;
@@ -586,15 +836,27 @@ constexpr int kMaxVocab = 1 << 30;
 constexpr int64_t kMaxGroups = ((int64_t)1 << 32) / 256 - 1;
 int capped_groups(int64_t g) { return (int)(g < kMaxGroups ? g : kMaxGroups); }
 
+// one thread a row has no use for alternatives: 16 lanes find them together
+// (8: a vector of 16-bit logits)
+bool by_rows(int rows, int vocab, int top) { return rows >= kRowsFrom && vocab >= 8 && vocab <= kRowsMax && top == 0; }
+int rows_groups(int rows) { return capped_groups(((int64_t)rows + kRowsThreads - 1) / kRowsThreads); }
+size_t rows_lds(int vocab) { return (size_t)kRowsThreads * rows_pitch(vocab) * sizeof(float); }
+
 template <typename T, bool MASK>
 void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
     if (pl.kind == 0) {
-        if (a.vocab <= 16 * kShortR)
-            hipLaunchKernelGGL((k_logprobs_short<T, 16, MASK>), dim3(capped_groups(((int64_t)a.rows + 15) / 16)),
-                               dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((k_logprobs_short<T, 64, MASK>), dim3(capped_groups(((int64_t)a.rows + 3) / 4)),
-                               dim3(256), 0, st, a);
+        const dim3 small(capped_groups(((int64_t)a.rows + 15) / 16)), wide(capped_groups(((int64_t)a.rows + 3) / 4));
+        if (by_rows(a.rows, a.vocab, a.top)) {
+            const dim3 grid(rows_groups(a.rows)), block(kRowsThreads);
+            constexpr int PER_16 = 16 / Vec<T>::N;
+            if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_rows<T, 2 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+            else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_rows<T, 3 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+            else hipLaunchKernelGGL((k_logprobs_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+        } else if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_short<T, 16, 3, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 64) hipLaunchKernelGGL((k_logprobs_short<T, 16, 4, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 128) hipLaunchKernelGGL((k_logprobs_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_logprobs_short<T, 64, 4, MASK>), wide, dim3(256), 0, st, a);
     } else if (pl.kind == 1) {
         const dim3 grid(capped_groups(((int64_t)a.rows + 3) / 4));
         if (a.top > 0) hipLaunchKernelGGL((k_logprobs_wave<T, MASK, true>), grid, dim3(256), 0, st, a);
@@ -609,12 +871,18 @@ void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
 template <typename T, bool MASK>
 void run_grad(const LpGradArgs& a, const LpPlan& pl, hipStream_t st) {
     if (pl.kind == 0) {
-        if (a.vocab <= 16 * kShortR)
-            hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, MASK>),
-                               dim3(capped_groups(((int64_t)a.rows + 15) / 16)), dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, MASK>),
-                               dim3(capped_groups(((int64_t)a.rows + 3) / 4)), dim3(256), 0, st, a);
+        const dim3 small(capped_groups(((int64_t)a.rows + 15) / 16)), wide(capped_groups(((int64_t)a.rows + 3) / 4));
+        if (by_rows(a.rows, a.vocab, a.top)) {
+            const dim3 grid(rows_groups(a.rows)), block(kRowsThreads);
+            constexpr int PER_16 = 16 / Vec<T>::N;
+            if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_grad_rows<T, 2 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+            else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_grad_rows<T, 3 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+            else hipLaunchKernelGGL((k_logprobs_grad_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
+        } else if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 3, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 64) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 4, MASK>), small, dim3(256), 0, st, a);
+        else if (a.vocab <= 128) hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 4, MASK>), wide, dim3(256), 0, st, a);
     } else {
         hipLaunchKernelGGL((k_logprobs_grad<T, MASK>), dim3((unsigned)((int64_t)a.rows * a.splits)), dim3(256), 0,
                            st, a);

@@ -526,16 +526,31 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # enum cfp_d
 
 def _need(ok, what):
     if not ok:
-        raise ValueError(what)
+        raise ValueError(what() if callable(what) else what)
+
+
+class _On:
+    """The device of the operands made current around a call (its current stream is the call's)."""
+
+    def __init__(self, device):
+        self._other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._other is not None:
+            self._other.__enter__()
+
+    def __exit__(self, *a):
+        if self._other is not None:
+            self._other.__exit__(*a)
 
 
 def _like(t, name, device, dtype, shape):
     """An optional contiguous argument's pointer, checked."""
     if t is None:
         return None
-    _need(t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-          f"{name}: a contiguous {dtype} tensor {tuple(shape)} on {device} expected, "
-          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _need(t.device == device and t.dtype == dtype and t.shape == shape and t.is_contiguous(),
+          lambda: f"{name}: a contiguous {dtype} tensor {shape} on {device} expected, "
+                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -577,13 +592,14 @@ def token_logprobs(logits, tokens, mask=None, top=0, stats=False):
     tok = _like(tokens, "tokens", dev, torch.int32, (rows,))
     _need(tok is not None, "tokens: expected")
     mp, ldm = _mask_of(mask, dev, rows, vocab)
-    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    lp = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty(rows, dtype=torch.float32, device=dev)
     ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if top > 0 else None
     tlp = torch.empty((rows, top), dtype=torch.float32, device=dev) if top > 0 else None
     st = torch.empty((rows, 3), dtype=torch.float32, device=dev) if stats else None
     need = lib().cfp_token_logprobs_workspace(rows, vocab, top)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
+    with _On(dev):
         _check(lib().cfp_token_logprobs(
             ptr, dtype, ld, rows, vocab, tok, mp, ldm, lp.data_ptr(), ent.data_ptr(), top,
             None if ids is None else ids.data_ptr(), None if tlp is None else tlp.data_ptr(),
@@ -613,7 +629,7 @@ def token_logprobs_backward(logits, tokens, stats, g_logprobs=None, g_entropy=No
     _need(out.device == dev and out.dtype == logits.dtype and out.shape == logits.shape,
           "out: the logits' shape, type and device expected")
     op, _, ldo = _rows_of(out, "out")
-    with torch.cuda.device(dev):
+    with _On(dev):
         _check(lib().cfp_token_logprobs_grad(ptr, dtype, ld, rows, vocab, tok, mp, ldm, st, g_lp, g_ent, top,
                                              ids, g_t, op, ldo, _stream()))
     return out
@@ -652,7 +668,7 @@ def orthogonalize(g, steps=5, coefs=None, eps=1e-7, products=0, out=None):
     c = _coefs_of(coefs, steps)
     need = lib().cfp_orthogonalize_workspace(batch, rows, cols, products)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _On(dev):
         _check(lib().cfp_orthogonalize(ptr, dtype, ld, stride, batch, rows, cols, steps,
                                        None if c is None else c.ctypes.data, eps, products, op, ldo, so,
                                        work.data_ptr(), need, _stream()))
@@ -676,7 +692,7 @@ def muon_update(w, g, momentum_buffer, lr, momentum=0.95, nesterov=True, weight_
     c = _coefs_of(coefs, steps)
     need = lib().cfp_orthogonalize_workspace(batch, rows, cols, products)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _On(dev):
         _check(lib().cfp_muon_update(ptr, g.data_ptr(), momentum_buffer.data_ptr(), ld, stride, batch, rows, cols,
                                      lr_dev, lr, momentum, 1 if nesterov else 0, weight_decay, scale, steps,
                                      None if c is None else c.ctypes.data, eps, products, work.data_ptr(), need,
