@@ -80,6 +80,20 @@ __device__ __forceinline__ void join(Sums& a, float m, float s, float u) {
 // All-reduce over 16 or 64 consecutive lanes in a tree of fixed shape.  Rotations inside rows of
 // 16 lanes ride on the addition itself (a shuffle through LDS a step instead: 27 us for 262 144
 // rows of 43 where this takes XXX).
+template <int D>
+__device__ __forceinline__ unsigned xor_lane(unsigned v) {
+    if (D == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);     // within quads
+    if (D == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);
+    if (D == 4)   // mirrored in eights, then in quads
+        return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true), 0x1b, 0xf, 0xf, true);
+    if (D == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);    // rotated by half a row
+    if (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+}
 template <int N>
 __device__ __forceinline__ float row_rotate(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + N, 0xf, 0xf, true));
@@ -92,8 +106,8 @@ __device__ __forceinline__ float reduce_lanes(float v, Op op) {
     v = op(v, row_rotate<2>(v));
     v = op(v, row_rotate<1>(v));
     if (WIDTH == 64) {
-        v = op(v, __shfl_xor(v, 16));
-        v = op(v, __shfl_xor(v, 32));
+        v = op(v, __uint_as_float(xor_lane<16>(__float_as_uint(v))));
+        v = op(v, __uint_as_float(xor_lane<32>(__float_as_uint(v))));
     }
     return v;
 }
@@ -112,104 +126,107 @@ __device__ __forceinline__ void join_lanes(Sums& a) {
 }
 
 // ---- the best `top` entries seen by one wavefront -----------------------------------
-// Lane i holds the entry of rank i (value, index), best first; index -1 marks a free place.
-// Order: larger value, then lower index.  An entry that beats the one of rank top - 1 goes to a
-// buffer in LDS; when that holds 64, they are sorted across the lanes (21 exchanges) and merged
-// with the list (6).  On values in random order the bar rises fast enough for the merges to
-// number about log4(entries / 64); one insertion at a time, about top * ln(entries / top) of
-// them and each as long as a few exchanges, took 34 us for 1 x 131 072 where this takes XXX.
-__device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// An entry is one 64-bit key, larger = better: the value's bits in unsigned order (0 and -0 the
+// same), then the complement of the index, so that equal values go to the lower index.  0 is a
+// free place; NaN and -inf never become keys.
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+    const unsigned u = __float_as_uint(v + 0.0f);
+    return (uint64_t)(u ^ ((unsigned)((int)u >> 31) | 0x80000000u)) << 32 | (unsigned)~i;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+    const unsigned h = (unsigned)(k >> 32);
+    return k == 0 ? -INFINITY : __uint_as_float(h & 0x80000000u ? h ^ 0x80000000u : ~h);
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return ~(int)(unsigned)k; }
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
+__device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
+    return (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)k, lane);
+}
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 template <int D>
-__device__ __forceinline__ unsigned xor_lane(unsigned v) {
-    if (D == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);
-    if (D == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);
-    if (D == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);
-    if (D < 32) return __builtin_amdgcn_ds_swizzle(v, (D << 10) | 0x1f);
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return threadIdx.x & 32 ? r[0] : r[1];
+__device__ __forceinline__ uint64_t xor_key(uint64_t k) {
+    return (uint64_t)xor_lane<D>((unsigned)(k >> 32)) << 32 | xor_lane<D>((unsigned)k);
 }
-struct Entry {
-    float v;
-    int i;
-};
-// keeps the better of this lane's and lane ^ D's entry where `better`, else the worse
-template <int D>
-__device__ __forceinline__ void exchange(Entry& e, bool better) {
-    const float ov = __uint_as_float(xor_lane<D>(__float_as_uint(e.v)));
-    const int oi = (int)xor_lane<D>((unsigned)e.i);
-    if (before(ov, oi, e.v, e.i) == better) { e.v = ov; e.i = oi; }
+// runs of 2 D become sorted, best first where `best_first` (alternating by bit 2 D of the lane),
+// from runs of D that alternate
+template <int STEP>
+__device__ __forceinline__ void merge_runs(uint64_t& k, bool best_first) {
+    const uint64_t other = xor_key<STEP>(k);
+    const bool keep_better = ((threadIdx.x & STEP) == 0) == best_first;
+    if ((other > k) == keep_better) k = other;
+    if constexpr (STEP > 1) merge_runs<STEP / 2>(k, best_first);
 }
-// runs of 2 D become sorted, alternately best first and last (by bit 2 D of the lane), from runs
-// of D that alternate
-template <int D, int STEP = D>
-__device__ __forceinline__ void merge_runs(Entry& e, bool best_first) {
-    const bool low = (threadIdx.x & STEP) == 0;
-    exchange<STEP>(e, low == best_first);
-    if constexpr (STEP > 1) merge_runs<D, STEP / 2>(e, best_first);
-}
+// Lane i of `key` holds the entry of rank i.  An entry that beats the one of rank top - 1 goes to
+// a buffer in LDS; when that holds 64, they are sorted across the lanes (21 exchanges) and merged
+// with the list (6).  On values in random order the bar rises fast enough for the merges to
+// number about log4(entries / 64); one insertion at a time, about top * ln(entries / top) of
+// them and each as long as a few exchanges, took 34 us for 1 x 131 072 where this takes XXX.
 constexpr int kBuffer = 128;   // of which 64 trigger a merge
 struct Best {
-    Entry e{-INFINITY, -1};
-    float last_v = -INFINITY;   // the entry of rank top - 1: what a newcomer has to beat
-    int last_i = -1;
+    uint64_t key = 0;
+    uint64_t last = 0;          // the entry of rank top - 1: what a newcomer has to beat
+    float last_v = -INFINITY;   // its value
     int waiting = 0;            // entries in the buffer; wave-uniform
-    float2* buffer;             // [kBuffer] of this wavefront
+    uint64_t* buffer;           // [kBuffer] of this wavefront
 
+    __device__ __forceinline__ static void sort(uint64_t& k, bool best_first) {
+        const int lane = threadIdx.x & 63;
+        merge_runs<1>(k, (lane & 2) == 0);
+        merge_runs<2>(k, (lane & 4) == 0);
+        merge_runs<4>(k, (lane & 8) == 0);
+        merge_runs<8>(k, (lane & 16) == 0);
+        merge_runs<16>(k, (lane & 32) == 0);
+        merge_runs<32>(k, best_first);
+    }
     // A bar for an empty list: every lane names the largest of the entries that it is about to
     // offer, and what does not reach the top-th largest of those cannot be among the best.  Of a
     // first tile about 1.2 top entries remain.
     __device__ __forceinline__ void set_bar(float largest, int top) {
-        if (last_v != -INFINITY) return;
-        Entry c{largest, (int)(threadIdx.x & 63)};
-        sort(c, true);
-        last_v = lane_value(c.v, top - 1);
-        last_i = last_v == -INFINITY ? -1 : 0x7fffffff;   // entries equal to the bar pass
-    }
-    __device__ __forceinline__ static void sort(Entry& c, bool best_first) {
-        const int lane = threadIdx.x & 63;
-        merge_runs<1>(c, (lane & 2) == 0);
-        merge_runs<2>(c, (lane & 4) == 0);
-        merge_runs<4>(c, (lane & 8) == 0);
-        merge_runs<8>(c, (lane & 16) == 0);
-        merge_runs<16>(c, (lane & 32) == 0);
-        merge_runs<32>(c, best_first);
+        if (last != 0) return;
+        if (top <= 8) {   // maxima one by one: 12 instructions each, the sort 190
+            float v = largest;
+            for (int k = 0; k < top; k++) {
+                last_v = max_lanes<64>(v);
+                const unsigned long long who = __ballot(v == last_v);
+                if ((int)(threadIdx.x & 63) == __ffsll(who) - 1) v = -INFINITY;
+            }
+            last = last_v > -INFINITY ? key_of(last_v, -1) : 0;   // index -1: entries equal to the bar pass
+            return;
+        }
+        uint64_t k = largest > -INFINITY ? key_of(largest, -1) : 0;
+        sort(k, true);
+        last = lane_key(k, top - 1);
+        last_v = key_value(last);
     }
     // the first 64 of the buffer into the list
     __device__ __forceinline__ void merge(int top) {
         const int lane = threadIdx.x & 63;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        Entry c{-INFINITY, -1};
-        if (lane < waiting) {
-            const float2 q = buffer[lane];
-            c = Entry{q.x, __float_as_int(q.y)};
-        }
+        uint64_t c = lane < waiting ? buffer[lane] : 0;
         if (waiting > 64) {   // the rest moves to the front
-            const float2 q = buffer[64 + lane];
+            const uint64_t rest = buffer[64 + lane];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            buffer[lane] = q;
+            buffer[lane] = rest;
         }
         waiting = waiting > 64 ? waiting - 64 : 0;
         sort(c, false);   // worst first: against the list it makes one bitonic run
-        if (before(c.v, c.i, e.v, e.i)) e = c;
-        merge_runs<32>(e, true);
-        last_v = lane_value(e.v, top - 1);
-        last_i = __builtin_amdgcn_readlane(e.i, top - 1);
+        if (c > key) key = c;
+        merge_runs<32>(key, true);
+        const uint64_t bar = lane_key(key, top - 1);
+        if (bar > last) { last = bar; last_v = key_value(bar); }
     }
-    // one entry a lane (wave-uniform call); entries of -inf and NaN never enter: the free
-    // places compare as (-inf, -1), which nothing of value -inf comes before
-    __device__ __forceinline__ void offer(float x, int idx, int top) {
-        const bool mine = before(x, idx, last_v, last_i);
+    // one entry a lane (wave-uniform call)
+    __device__ __forceinline__ void offer(float x, int idx, int top) { offer(x > -INFINITY ? key_of(x, idx) : 0, top); }
+    __device__ __forceinline__ void offer(uint64_t k, int top) {
+        const bool mine = k > last;
         const unsigned long long who = __ballot(mine);
         if (who == 0) return;
-        if (mine) {
-            const int at = waiting + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
-            buffer[at] = make_float2(x, __int_as_float(idx));
-        }
+        if (mine) buffer[waiting + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0))] = k;
         waiting += __popcll(who);
         if (waiting >= 64) merge(top);
     }
@@ -233,7 +250,7 @@ struct LpArgs {
     float* stats;          // [rows][3] or null
     int splits, chunk;     // entries per split, a multiple of 8
     f4* part;              // [rows][splits] (m, s, u, -)
-    float2* part_top;      // [rows][splits][top] (value, index bits)
+    uint64_t* part_top;    // [rows][splits][top] keys
 };
 
 // Outputs of one row from its sums; called by one lane.  xt: the given token's logit, -inf
@@ -254,11 +271,13 @@ __device__ __forceinline__ void write_row(const LpArgs& a, int row, const Sums& 
         st[2] = h;
     }
 }
-__device__ __forceinline__ void write_top(const LpArgs& a, int row, const Sums& z, int rank, float v, int i) {
+__device__ __forceinline__ void write_top(const LpArgs& a, int row, const Sums& z, int rank, uint64_t key) {
+    const float v = key_value(key);
+    const int i = key_index(key);
     const size_t o = (size_t)row * a.top + rank;
     const bool bad = z.s != z.s;   // NaN or +inf among the allowed entries
-    a.ids[o] = bad ? -1 : i;
-    a.top_lp[o] = bad ? NAN : i < 0 ? -INFINITY : (v - z.m) - logf(z.s);
+    a.ids[o] = bad ? -1 : i;   // a free place has index -1
+    a.top_lp[o] = bad ? NAN : key == 0 ? -INFINITY : (v - z.m) - logf(z.s);
 }
 template <typename T>
 __device__ __forceinline__ float token_logit(const LpArgs& a, int row, int tok) {
@@ -268,34 +287,69 @@ __device__ __forceinline__ float token_logit(const LpArgs& a, int row, int tok) 
     return x;
 }
 
-// ---- short rows: L lanes a row, R <= 4 entries a lane ----------------------------------
-// Each load instruction of a lane group covers L consecutive entries of its row.  No online
-// rescaling: the row sits in registers.  kShortMax entries at most.
-constexpr int kShortMax = 64 * 4;
-template <typename T, int L, int R, bool MASK>
+// ---- short rows: L lanes a row, Q 16-byte vectors a lane ----------------------------------
+// The row sits in registers: the maximum first, then the exponentials, no rescaling.  The last
+// vector of a row is moved back to end with it; the entries it shares with the one before count
+// once (as -inf here).
+constexpr int kShortBytes = 2048;   // of a row: 64 lanes, two vectors each
+template <typename T, int L, int Q, bool MASK>
+__device__ __forceinline__ void load_short(const T* x, const uint8_t* mask, int vocab, int sub, float (&v)[Q][Vec<T>::N],
+                                           int (&first)[Q]) {
+    constexpr int N = Vec<T>::N;
+    if (vocab < N) {   // not even one vector
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            first[q] = q == 0 && sub == 0 ? 0 : vocab;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                v[q][j] = -INFINITY;
+                if (first[q] + j < vocab && (!MASK || mask[j])) v[q][j] = to_f32(x[j]);
+            }
+        }
+        return;
+    }
+    Vec<T> raw[Q];
+    uint8_t mk[Q][N];
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const int i = (q * L + sub) * N;
+        first[q] = min(i, vocab - N);
+        raw[q] = load_vec(x + first[q]);   // lanes behind the row repeat its last vector
+        if (MASK) __builtin_memcpy(mk[q], mask + first[q], N);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const int i = (q * L + sub) * N;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            v[q][j] = first[q] + j < i || (MASK && mk[q][j] == 0) ? -INFINITY : to_f32(raw[q].v[j]);
+    }
+}
+template <typename T, int L, int Q, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
+    constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
     for (int row0 = (int)blockIdx.x * per; row0 < a.rows; row0 += (int)gridDim.x * per) {
         const int row = row0 + (int)threadIdx.x / L;
         const bool live = row < a.rows;
         const int r = live ? row : a.rows - 1;
-        const T* x = (const T*)a.x + (size_t)r * a.ld;
-        const uint8_t* mask = MASK ? a.mask + (size_t)r * a.ld_mask : nullptr;
         const int tok = a.tok[r];
         const float xt = token_logit<T>(a, r, tok);
-        float v[R];
+        float v[Q][N];
+        int first[Q];
+        load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
+                                  a.vocab, sub, v, first);
         Sums z;
 #pragma unroll
-        for (int j = 0; j < R; j++) {
-            const int i = j * L + sub;
-            v[j] = -INFINITY;
-            if (i < a.vocab && (!MASK || mask[i])) v[j] = to_f32(x[i]);
-            z.m = fmaxf(z.m, v[j]);
-        }
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) z.m = fmaxf(z.m, v[q][j]);
         z.m = max_lanes<L>(z.m);
 #pragma unroll
-        for (int j = 0; j < R; j++) add_entry(z, v[j]);
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
         z.s = sum_lanes<L>(z.s);
         z.u = sum_lanes<L>(z.u);
         if (live && sub == 0) write_row(a, row, z, tok, xt);
@@ -303,18 +357,26 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
             float bv = -INFINITY;
             int bi = -1;
 #pragma unroll
-            for (int j = 0; j < R; j++)   // ascending index: ties keep the first
-                if (v[j] > bv) { bv = v[j]; bi = j * L + sub; }
+            for (int q = 0; q < Q; q++)
 #pragma unroll
-            for (int d = L / 2; d > 0; d >>= 1) {
-                const float ov = __shfl_xor(bv, d, L);
-                const int oi = __shfl_xor(bi, d, L);
-                if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+                for (int j = 0; j < N; j++)   // ascending index: ties keep the first
+                    if (v[q][j] > bv) { bv = v[q][j]; bi = first[q] + j; }
+            uint64_t best = bi >= 0 ? key_of(bv, bi) : 0;
+            best = larger(best, xor_key<1>(best));
+            best = larger(best, xor_key<2>(best));
+            best = larger(best, xor_key<4>(best));
+            best = larger(best, xor_key<8>(best));
+            if (L == 64) {
+                best = larger(best, xor_key<16>(best));
+                best = larger(best, xor_key<32>(best));
             }
+            bi = key_index(best);
 #pragma unroll
-            for (int j = 0; j < R; j++)
-                if (j * L + sub == bi) v[j] = -INFINITY;
-            if (live && sub == 0) write_top(a, row, z, k, bv, bi);
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (first[q] + j == bi) v[q][j] = -INFINITY;
+            if (live && sub == 0) write_top(a, row, z, k, best);
         }
     }
 }
@@ -398,7 +460,7 @@ constexpr int kU = 4;
 // 4096 x 131 072 instead of XXX.)
 constexpr int kLaneBytes = 80;
 struct TopSpace {
-    float2 buffer[kBuffer];
+    uint64_t buffer[kBuffer];
     __align__(16) unsigned char tile[64 * kLaneBytes];
 };
 template <typename T>
@@ -429,12 +491,8 @@ __device__ __forceinline__ void offer_tile(const float (&v)[kU][Vec<T>::N], floa
             todo &= todo - 1;   // 0 stays 0
         }
         float x = -INFINITY;
-        int idx = 0;   // not below -1: (-inf, -2) would come before a free place
-        if (src >= 0) {
-            x = to_f32(*reinterpret_cast<const T*>(tile + src * kLaneBytes + 16 * q + j * (int)sizeof(T)));
-            idx = base + q * stride + (lane0 + src) * N + j;
-        }
-        best.offer(x, idx, top);
+        if (src >= 0) x = to_f32(*reinterpret_cast<const T*>(tile + src * kLaneBytes + 16 * q + j * (int)sizeof(T)));
+        best.offer(x, base + q * stride + (lane0 + src) * N + j, top);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -484,13 +542,15 @@ __device__ __forceinline__ void stream_row(const T* x, const uint8_t* mask, int 
         float tm = v[0][0];
 #pragma unroll
         for (int q = 0; q < kU; q++)
+            if (q == 0 || base + q * STRIDE < hi)   // a partial tile has fewer
 #pragma unroll
-            for (int j = 0; j < N; j++) tm = fmaxf(tm, v[q][j]);
+                for (int j = 0; j < N; j++) tm = fmaxf(tm, v[q][j]);
         if (tm > z.m) raise_max(z, tm);
 #pragma unroll
         for (int q = 0; q < kU; q++)
+            if (q == 0 || base + q * STRIDE < hi)
 #pragma unroll
-            for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
+                for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
         if (TOP) offer_tile<T>(v, tm, base, STRIDE, t - (int)(threadIdx.x & 63), space->tile, best, top);
     }
 }
@@ -515,7 +575,7 @@ __global__ __launch_bounds__(256) void k_logprobs_wave(LpArgs a) {
         join_lanes(z);
         if (lane == 0) write_row(a, row, z, tok, xt);
         if (TOP) best.finish(a.top);
-        if (TOP && lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
+        if (TOP && lane < a.top) write_top(a, row, z, lane, best.key);
     }
 }
 
@@ -526,7 +586,7 @@ template <typename T, bool MASK, bool TOP>
 __global__ __launch_bounds__(64 * kWaves) void k_logprobs_group(LpArgs a) {
     __shared__ float zs[kWaves][3];
     __shared__ TopSpace spaces[TOP ? kWaves : 1];
-    __shared__ float2 lists[TOP ? kWaves : 1][kMaxTop];
+    __shared__ uint64_t lists[TOP ? kWaves : 1][kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
     const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
@@ -541,32 +601,29 @@ __global__ __launch_bounds__(64 * kWaves) void k_logprobs_group(LpArgs a) {
     join_lanes(z);
     if (lane == 0) { zs[wave][0] = z.m; zs[wave][1] = z.s; zs[wave][2] = z.u; }
     if (TOP) best.finish(a.top);
-    if (TOP && wave > 0 && lane < a.top) lists[wave][lane] = make_float2(best.e.v, __int_as_float(best.e.i));
+    if (TOP && wave > 0 && lane < a.top) lists[wave][lane] = best.key;
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
     for (int w = 1; w < kWaves; w++) join(z, zs[w][0], zs[w][1], zs[w][2]);
     if (TOP) {
-        for (int w = 1; w < kWaves; w++) {
-            const float2 e = lane < a.top ? lists[w][lane] : make_float2(-INFINITY, __int_as_float(-1));
-            best.offer(e.x, __float_as_int(e.y), a.top);
-        }
+        for (int w = 1; w < kWaves; w++) best.offer(lane < a.top ? lists[w][lane] : 0, a.top);
         best.finish(a.top);
     }
     if (a.splits == 1) {
         if (lane == 0) write_row(a, row, z, tok, xt);
-        if (TOP && lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
+        if (TOP && lane < a.top) write_top(a, row, z, lane, best.key);
         return;
     }
     const size_t o = (size_t)row * a.splits + split;
     if (lane == 0) a.part[o] = f4{z.m, z.s, z.u, 0.0f};
-    if (TOP && lane < a.top) a.part_top[o * a.top + lane] = make_float2(best.e.v, __int_as_float(best.e.i));
+    if (TOP && lane < a.top) a.part_top[o * a.top + lane] = best.key;
 }
 
 // One wavefront a row: the parts of its splits in ascending order of lane, then the tree.
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs a) {
-    __shared__ float2 buffer[kBuffer];
+    __shared__ uint64_t buffer[kBuffer];
     const int lane = threadIdx.x, row = (int)blockIdx.x;
     const int tok = a.tok[row];
     const float xt = token_logit<T>(a, row, tok);
@@ -580,15 +637,12 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LpArgs a) {
     if (a.top > 0) {
         Best best;
         best.buffer = buffer;
-        best.set_bar(lane < a.splits ? a.part_top[((size_t)row * a.splits + lane) * a.top].x : -INFINITY, a.top);
         const int total = a.splits * a.top;
-        for (int o = 0; o < total; o += 64) {
-            float2 e = make_float2(-INFINITY, __int_as_float(-1));
-            if (o + lane < total) e = a.part_top[(size_t)row * total + o + lane];
-            best.offer(e.x, __float_as_int(e.y), a.top);
-        }
+        const uint64_t* keys = a.part_top + (size_t)row * total;
+        best.set_bar(lane < a.splits ? key_value(keys[lane * a.top]) : -INFINITY, a.top);
+        for (int o = 0; o < total; o += 64) best.offer(o + lane < total ? keys[o + lane] : 0, a.top);
         best.finish(a.top);
-        if (lane < a.top) write_top(a, row, z, lane, best.e.v, best.e.i);
+        if (lane < a.top) write_top(a, row, z, lane, best.key);
     }
 }
 
@@ -645,44 +699,56 @@ __device__ __forceinline__ void row_grad(const LpGradArgs& a, int row, float wei
     r.weight = weight;
     r.g_ent = a.g_ent ? a.g_ent[row] : 0.0f;
 }
-template <typename T, int L, int R, bool MASK>
+template <typename T, int L, int Q, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_grad_short(LpGradArgs a) {
+    constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
     for (int row0 = (int)blockIdx.x * per; row0 < a.rows; row0 += (int)gridDim.x * per) {
         const int row = row0 + (int)threadIdx.x / L;
         const bool live = row < a.rows;
         const int r = live ? row : a.rows - 1;
-        const T* x = (const T*)a.x + (size_t)r * a.ld;
-        const uint8_t* mask = MASK ? a.mask + (size_t)r * a.ld_mask : nullptr;
-        float v[R], d[R];
+        float v[Q][N], d[Q][N];
+        int first[Q];
+        load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
+                                  a.vocab, sub, v, first);
 #pragma unroll
-        for (int j = 0; j < R; j++) {
-            const int i = j * L + sub;
-            v[j] = -INFINITY;
-            if (i < a.vocab && (!MASK || mask[i])) v[j] = to_f32(x[i]);
-            d[j] = 0.0f;
-        }
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) d[q][j] = 0.0f;
         // the named entries: whose lane holds an allowed one takes its gradient
         float weight = 0.0f;
-        for (int j = 0; j <= a.top; j++) {
-            if (j == 0 && !a.g_lp) continue;
-            const int i = j == 0 ? a.tok[r] : a.ids[(size_t)r * a.top + j - 1];
-            const float g = j == 0 ? a.g_lp[r] : a.g_top[(size_t)r * a.top + j - 1];
+        for (int k = 0; k <= a.top; k++) {
+            if (k == 0 && !a.g_lp) continue;
+            const int i = k == 0 ? a.tok[r] : a.ids[(size_t)r * a.top + k - 1];
+            const float g = k == 0 ? a.g_lp[r] : a.g_top[(size_t)r * a.top + k - 1];
             if (i >= a.vocab && sub == 0) weight = NAN;
 #pragma unroll
-            for (int q = 0; q < R; q++)
-                if (q * L + sub == i && !(v[q] == -INFINITY)) { d[q] += g; weight += g; }
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (first[q] + j == i && !(v[q][j] == -INFINITY)) { d[q][j] += g; weight += g; }
         }
         RowGrad rg;
         row_grad(a, r, sum_lanes<L>(weight), rg);
         T* dx = (T*)a.dx + (size_t)r * a.ld_dx;
 #pragma unroll
-        for (int j = 0; j < R; j++) {
-            const int i = j * L + sub;
-            const bool on = !rg.none && !(v[j] == -INFINITY);
-            // every load of this row was used above: the row may be overwritten in place
-            if (live && i < a.vocab) dx[i] = (T)(on ? rg.at(v[j]) + d[j] : 0.0f);
+        for (int q = 0; q < Q; q++) {
+            // every load of this row was used above: the row may be overwritten in place.  Each
+            // entry is stored by the lane that it counts for.
+            const int i = (q * L + sub) * N;
+            Vec<T> out;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const bool on = !rg.none && !(v[q][j] == -INFINITY);
+                out.v[j] = (T)(on ? rg.at(v[q][j]) + d[q][j] : 0.0f);
+            }
+            if (!live) continue;
+            if (i + N <= a.vocab) store_vec(dx + i, out);
+            else
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (first[q] + j >= i && first[q] + j < a.vocab) dx[first[q] + j] = out.v[j];
         }
     }
 }
@@ -804,13 +870,15 @@ struct LpPlan {
     int kind;     // 0 short, 1 a wavefront a row, 2 a workgroup a split
     int splits, chunk;
 };
-// Rows of up to 256 entries sit in the registers of 16 or 64 lanes.  Longer ones are streamed: by
+// Rows of up to 2 KiB sit in the registers of 16 or 64 lanes (1 KiB from four alternatives on, 512
+// bytes from nine on: finding them one by one costs 70 to 110 instructions each there, sorting
+// candidates about 500 once; 100 000 x 300 with 5: 99 us against 125).  Longer ones are streamed: by
 // a wavefront each where there are enough rows to fill the machine that way (256 CUs, 16
 // wavefronts each) and a row is not so long that its last wavefronts run alone; by a workgroup
 // each otherwise, split further until about four workgroups a CU run, none with less than 4096
 // entries (one tile of 16-bit loads is 8192, and a second launch joins the parts).
-LpPlan plan_forward(int rows, int vocab) {
-    if (vocab <= kShortMax) return {0, 1, 0};
+LpPlan plan_forward(int rows, int vocab, int bytes, int top) {
+    if ((int64_t)vocab * bytes <= (top < 4 ? kShortBytes : top <= 8 ? kShortBytes / 2 : kShortBytes / 4)) return {0, 1, 0};
     if (rows >= 4096 && vocab <= 8192) return {1, 1, 0};
     const int want = rows >= 512 ? 1 : (1024 + rows - 1) / rows;
     const int most = (vocab + 4095) / 4096;
@@ -820,15 +888,15 @@ LpPlan plan_forward(int rows, int vocab) {
     return {2, splits, chunk};
 }
 // the gradient's parts are independent: 16384 entries a workgroup at most, 2048 at least
-LpPlan plan_grad(int rows, int vocab) {
-    if (vocab <= kShortMax) return {0, 1, 0};
+LpPlan plan_grad(int rows, int vocab, int bytes) {
+    if ((int64_t)vocab * bytes <= kShortBytes) return {0, 1, 0};
     int splits = (vocab + 16383) / 16384;
     while ((int64_t)rows * splits < 2048 && (vocab + splits - 1) / splits > 2048) splits *= 2;
     const int chunk = ((vocab + splits - 1) / splits + 7) / 8 * 8;
     return {2, (vocab + chunk - 1) / chunk, chunk};
 }
 size_t part_bytes(int rows, int splits, int top) {
-    return splits == 1 ? 0 : (size_t)rows * splits * (sizeof(f4) + (size_t)top * sizeof(float2));
+    return splits == 1 ? 0 : (size_t)rows * splits * (sizeof(f4) + (size_t)top * sizeof(uint64_t));
 }
 
 constexpr int kMaxVocab = 1 << 30;
@@ -852,11 +920,13 @@ void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
             if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_rows<T, 2 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
             else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_rows<T, 3 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
             else hipLaunchKernelGGL((k_logprobs_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
-        } else if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_short<T, 16, 3, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 64) hipLaunchKernelGGL((k_logprobs_short<T, 16, 4, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 128) hipLaunchKernelGGL((k_logprobs_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_logprobs_short<T, 64, 4, MASK>), wide, dim3(256), 0, st, a);
+        } else {
+            const int vectors = (a.vocab + Vec<T>::N - 1) / Vec<T>::N;   // 16 lanes up to 32 of them
+            if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_short<T, 16, 1, MASK>), small, dim3(256), 0, st, a);
+            else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
+            else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_short<T, 64, 1, MASK>), wide, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_logprobs_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+        }
     } else if (pl.kind == 1) {
         const dim3 grid(capped_groups(((int64_t)a.rows + 3) / 4));
         if (a.top > 0) hipLaunchKernelGGL((k_logprobs_wave<T, MASK, true>), grid, dim3(256), 0, st, a);
@@ -878,11 +948,13 @@ void run_grad(const LpGradArgs& a, const LpPlan& pl, hipStream_t st) {
             if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_grad_rows<T, 2 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
             else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_grad_rows<T, 3 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
             else hipLaunchKernelGGL((k_logprobs_grad_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
-        } else if (a.vocab <= 32) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 48) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 3, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 64) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 4, MASK>), small, dim3(256), 0, st, a);
-        else if (a.vocab <= 128) hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 4, MASK>), wide, dim3(256), 0, st, a);
+        } else {
+            const int vectors = (a.vocab + Vec<T>::N - 1) / Vec<T>::N;   // 16 lanes up to 32 of them
+            if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 1, MASK>), small, dim3(256), 0, st, a);
+            else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
+            else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 1, MASK>), wide, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+        }
     } else {
         hipLaunchKernelGGL((k_logprobs_grad<T, MASK>), dim3((unsigned)((int64_t)a.rows * a.splits)), dim3(256), 0,
                            st, a);
@@ -917,7 +989,7 @@ extern "C" {
 
 size_t cfp_token_logprobs_workspace(int rows, int vocab, int top) {
     if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab || top < 0 || top > kMaxTop) return 0;
-    return part_bytes(rows, plan_forward(rows, vocab).splits, top);
+    return part_bytes(rows, plan_forward(rows, vocab, 4, top).splits, top);   // splits do not depend on the type
 }
 
 int cfp_token_logprobs(const void* d_logits, int dtype, int64_t ld, int rows, int vocab, const int32_t* d_tokens,
@@ -928,7 +1000,7 @@ int cfp_token_logprobs(const void* d_logits, int dtype, int64_t ld, int rows, in
     if (rows == 0) return 0;
     CFP_REQUIRE(d_logprobs, "cfp_token_logprobs: NULL output");
     CFP_REQUIRE(top == 0 || (d_top_ids && d_top_logprobs), "cfp_token_logprobs: top = %d needs both arrays of alternatives", top);
-    const LpPlan pl = plan_forward(rows, vocab);
+    const LpPlan pl = plan_forward(rows, vocab, (int)elem_bytes(dtype), top);
     CFP_REQUIRE(pl.kind < 2 || (int64_t)rows * pl.splits <= kMaxGroups, "cfp_token_logprobs: %d rows of %d are more than one launch holds",
                 rows, vocab);
     const size_t need = part_bytes(rows, pl.splits, top);
@@ -941,7 +1013,7 @@ int cfp_token_logprobs(const void* d_logits, int dtype, int64_t ld, int rows, in
     a.stats = d_stats;
     a.splits = pl.splits; a.chunk = pl.chunk;
     a.part = (f4*)d_work;
-    a.part_top = need ? (float2*)((f4*)d_work + (size_t)rows * pl.splits) : nullptr;
+    a.part_top = need ? (uint64_t*)((f4*)d_work + (size_t)rows * pl.splits) : nullptr;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == CFP_F32) { d_mask ? run_forward<float, true>(a, pl, st) : run_forward<float, false>(a, pl, st); }
     else if (dtype == CFP_BF16) { d_mask ? run_forward<__bf16, true>(a, pl, st) : run_forward<__bf16, false>(a, pl, st); }
@@ -968,7 +1040,7 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
     const char* y1 = y0 + ((size_t)(rows - 1) * ld_dlogits + vocab) * elem_bytes(dtype);
     CFP_REQUIRE(y0 >= x1 || x0 >= y1 || (x0 == y0 && (ld == ld_dlogits || rows == 1)),
                 "cfp_token_logprobs_grad: the gradient may replace the logits, with the same stride, but not overlap them otherwise");
-    const LpPlan pl = plan_grad(rows, vocab);
+    const LpPlan pl = plan_grad(rows, vocab, (int)elem_bytes(dtype));
     CFP_REQUIRE(pl.kind < 2 || (int64_t)rows * pl.splits <= kMaxGroups, "cfp_token_logprobs_grad: %d rows of %d are more than one launch holds",
                 rows, vocab);
     LpGradArgs a{};
