@@ -140,8 +140,6 @@ __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) 
     __shared__ float tile[64][65];
     __shared__ double ws[4];
     const int bt = blockIdx.z;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < a.groups; i += 256) s += a.part[(size_t)bt * a.groups + i];
     const size_t base = (size_t)bt * a.stride;
     // G's rows and columns, padded
     const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;
@@ -156,6 +154,8 @@ __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) 
             u[k] = a.nesterov ? u[k] + a.beta * m : m;
         }
     }
+    double s = 0.0;
+    for (int i = threadIdx.x; i < a.groups; i += 256) s += a.part[(size_t)bt * a.groups + i];
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -263,12 +263,16 @@ struct MulArgs {
     size_t l_batch, r_batch; // values a matrix
     int stages;              // of 32 values; even
     int tiles_i;
-    unsigned row_len;
-    uint64_t row_inv;
+    unsigned row_len;        // tiles of a pair of rows (symmetric products) or of a band of four
+    uint64_t row_inv;        // ceil(2^32 / row_len)
+    int by_xcd;              // 0, or the matrices of the batch where one XCD takes each
     Work w;
     int cur;                 // y[cur] is X transposed before the step
     float a, b, c;
     OutArgs out;
+    // X X^T of few tiles and many stages: the stages shared out over `splits` workgroups a tile
+    int splits;
+    f4* part;                // [batch][tile][split][4 wavefronts][4][64 lanes]
 };
 __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -317,10 +321,134 @@ __device__ __forceinline__ u2 transpose_quad(u2 w, int c) {
     return low ? u2{r[0], got} : u2{got, r[1]};
 }
 
+// ---- what becomes of a 32 x 32 block of the product -------------------------------------
+// A lane holds column n32 of the block, rows 8 q + 4 half + 0..3 (q = 0..3).  Transposed
+// matrices (rows j) are read and written 16 bytes a lane: lanes n32 and n32 + 32 hold
+// neighbouring 8-byte pieces, of q = 2 t and 2 t + 1, and swap two of the four dwords.
+// What is added to the product: X transposed (with its lo part), or A.
+struct Addend {
+    u4 v[2][2];   // [t][hi, lo]
+};
+template <int P, int MODE>
+__device__ __forceinline__ void load_addend(const MulArgs& g, size_t bt, int ib, int jb, int lane, Addend& a) {
+    if (MODE == kGram) return;
+    const int j = jb + (lane & 31), half = lane >> 5;
+    const size_t mat_y = bt * g.w.np * (size_t)g.w.ldm;
+    const _Float16* m = MODE == kPoly ? g.w.a + bt * g.w.mp * (size_t)g.w.ldm : g.w.y[g.cur] + mat_y;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const size_t o = at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
+        a.v[t][0] = *reinterpret_cast<const u4*>(m + o);
+        if (P == 3) a.v[t][1] = *reinterpret_cast<const u4*>(m + o + kLo);
+        else if (MODE != kPoly) a.v[t][1] = *reinterpret_cast<const u4*>(g.w.y_lo + mat_y + o);
+    }
+}
+template <int P, int MODE>
+__device__ __forceinline__ void finish_block(const MulArgs& g, size_t bt, const f16v& acc, Addend& add, int ib, int jb, int lane,
+                                             bool diagonal, float (*out_stage)[33]) {
+    constexpr bool SYM = MODE == kGram || MODE == kPoly, HAS_LO = P == 3 || !SYM;
+    const int n32 = lane & 31, half = lane >> 5, quad = lane & 3, j = jb + n32;
+    const size_t mat_a = bt * g.w.mp * (size_t)g.w.ldm, mat_y = bt * g.w.np * (size_t)g.w.ldm;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        if (MODE != kGram) {
+            swap_halves(add.v[t][0]);
+            if (HAS_LO) swap_halves(add.v[t][1]);
+        }
+        u4 hi_out, lo_out;   // dwords 0, 1: q = 2 t; 2, 3: q = 2 t + 1
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int q = 2 * t + u;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[e] = acc[4 * q + e];
+                float x = 0.0f;
+                if (MODE != kGram) {
+                    x = half_of(add.v[t][0], 4 * u + e);
+                    if (HAS_LO) x += half_of(add.v[t][1], 4 * u + e);
+                }
+                if (MODE == kGram) v[e] *= kScaleA / (kScaleX * kScaleX);
+                else if (MODE == kPoly) v[e] = g.b * x + (g.c / kScaleA) * v[e];
+                else v[e] = g.a * x + v[e] * (1.0f / kScaleA);
+            }
+            if (MODE == kLast) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) out_stage[8 * q + 4 * half + e][n32] = v[e] * (1.0f / kScaleX);
+                continue;
+            }
+            h4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                _Float16 p, r;
+                split_hl(v[e], p, r);
+                hi[e] = p; lo[e] = r;
+            }
+            const u2 hw = __builtin_bit_cast(u2, hi), lw = __builtin_bit_cast(u2, lo);
+            hi_out[2 * u] = hw[0]; hi_out[2 * u + 1] = hw[1];
+            lo_out[2 * u] = lw[0]; lo_out[2 * u + 1] = lw[1];
+            // row-major: four lanes exchange their columns, one row of four entries each
+            _Float16* to = MODE == kGram ? g.w.a + mat_a : MODE == kPoly ? g.w.b + mat_a
+                                                                         : g.w.x + bt * g.w.mp * (size_t)g.w.ldn;
+            to += at<P>(ib + 8 * q + 4 * half + quad, SYM ? g.w.ldm : g.w.ldn, jb + (n32 & 28));
+            *reinterpret_cast<u2*>(to) = transpose_quad(hw, quad);
+            if (P == 3) *reinterpret_cast<u2*>(to + kLo) = transpose_quad(lw, quad);
+        }
+        if (MODE == kLast) continue;
+        // a tile on the diagonal holds both halves itself, and has stored them
+        if (SYM && diagonal) continue;
+        const size_t o = at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
+        _Float16* to = SYM ? (MODE == kGram ? g.w.a : g.w.b) + mat_a : g.w.y[g.cur ^ 1] + mat_y;
+        swap_halves(hi_out);
+        *reinterpret_cast<u4*>(to + o) = hi_out;
+        if (HAS_LO) {
+            swap_halves(lo_out);
+            *reinterpret_cast<u4*>(P == 3 ? to + o + kLo : g.w.y_lo + mat_y + o) = lo_out;
+        }
+    }
+}
+// rows of 32 values of the result, two a wavefront and instruction, eight in flight
+__device__ __forceinline__ void write_result(const OutArgs& o, size_t bt, int ib, int jb, int lane, const float (*out_stage)[33]) {
+#pragma unroll 1
+    for (int b = 0; b < 2; b++) {
+        const int n32 = lane & 31, p0 = 16 * b + (lane >> 5);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = o.tall ? out_stage[n32][p0 + 2 * k] : out_stage[p0 + 2 * k][n32];
+        put_rows(o, bt * o.stride, (o.tall ? jb : ib) + p0, (o.tall ? ib : jb) + n32, v);
+    }
+}
+
 // f(0), f(1), ... with compile-time numbers (a loop of 48 steps is not unrolled whole)
 template <class Fn, int... I>
 __device__ __forceinline__ void each(std::integer_sequence<int, I...>, Fn&& f) {
     (f(std::integral_constant<int, I>{}), ...);
+}
+
+// Tile t of `total`.  In scalar arithmetic throughout (addresses of copies are scalar operands):
+// t / d as t * ceil(2^32 / d) / 2^32, exact while t * d < 2^32.
+template <bool SYM>
+__device__ __forceinline__ void tile_of(const MulArgs& g, unsigned t, unsigned total, int& ti, int& tj) {
+    // Workgroups go to the eight XCDs in turn; an XCD takes a run of tiles, which share panels in its
+    // L2 (2048 x 8192 bf16, all steps: 992 us instead of 1040).
+    if (!g.by_xcd) {
+        const unsigned x = t % 8, q = total / 8, r = total % 8;
+        t = x * q + (x < r ? x : r) + t / 8;
+    }
+    if (SYM) {
+        // tiles on and above the diagonal: row r and row n - 1 - r have n + 1 of them together
+        const unsigned row = (unsigned)((t * g.row_inv) >> 32), col = t - row * g.row_len;
+        const int n = g.tiles_i, r = (int)row, c = (int)col;
+        ti = c < n - r ? r : n - 1 - r;
+        tj = c < n - r ? r + c : c - 1;
+    } else {
+        // bands of four tile rows, column by column
+        const unsigned band = (unsigned)((t * g.row_inv) >> 32), rest = t - band * g.row_len;
+        const unsigned rows = (unsigned)g.tiles_i - 4 * band;   // of the last band: 1 to 4
+        const unsigned col = rows >= 4 ? rest >> 2 : rows == 3 ? (rest * 43691u) >> 17 : rows == 2 ? rest >> 1 : rest;
+        ti = (int)(4 * band + rest - col * (rows >= 4 ? 4 : rows));
+        tj = (int)col;
+    }
 }
 
 // 2 x 2 wavefronts of F x F blocks of 32 x 32 (tiles of 64 F).  A stage is SUB times 32 values of
@@ -342,26 +470,25 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
     constexpr int NM = (P == 3 ? 3 : 1) * F * F, NR = 2 * PL * F;
     __shared__ __align__(1024) unsigned char lds[R][SUB][2 * T * 64];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
-    // Tile of this workgroup; per_row is in scalar arithmetic throughout (addresses of copies are
-    // scalar operands): t / d as t * ceil(2^32 / d) / 2^32, exact while t * d < 2^32.
-    const unsigned t = blockIdx.x, row = (unsigned)((t * g.row_inv) >> 32), col = t - row * g.row_len;
+    // by_xcd: blockIdx.y and the residue of blockIdx.x (the XCD) name the matrix
+    const unsigned tile = g.by_xcd ? blockIdx.x / 8 : blockIdx.x;
+    const size_t bt = g.by_xcd ? blockIdx.y * 8 + blockIdx.x % 8 : blockIdx.y;
+    if (g.by_xcd && (int)bt >= g.by_xcd) return;
     int ti, tj;
-    if (MODE == kGram || MODE == kPoly) {
-        // tiles on and above the diagonal: row r and row n - 1 - r have n + 1 of them together
-        const int n = g.tiles_i, r = (int)row, c = (int)col;
-        ti = c < n - r ? r : n - 1 - r;
-        tj = c < n - r ? r + c : c - 1;
-    } else {
-        ti = (int)col;
-        tj = (int)row;
-    }
-    const size_t bt = blockIdx.y;
+    tile_of<SYM>(g, tile, g.by_xcd ? gridDim.x / 8 : gridDim.x, ti, tj);
     const int i0 = ti * T, j0 = tj * T;
     // this wave's pieces of stage 0: F of the L side, F of the R side
     const _Float16* from[2] = {g.l + bt * g.l_batch + (size_t)(i0 / 16 + wave) * (g.ldl >> 5) * kPiece,
                                g.r + bt * g.r_batch + (size_t)(j0 / 16 + wave) * (g.ldr >> 5) * kPiece};
     const size_t hop[2] = {(size_t)WAVES * (g.ldl >> 5) * kPiece, (size_t)WAVES * (g.ldr >> 5) * kPiece};
     const unsigned voff = (unsigned)((lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16);
+    constexpr bool SPLIT = MODE == kGram && F == 1;
+    int first = 0, last = g.stages / SUB - 1;   // stages of this workgroup
+    if (SPLIT) {
+        const unsigned all = (unsigned)(last + 1), z = blockIdx.z;
+        first = (int)(all * z / (unsigned)g.splits);
+        last = (int)(all * (z + 1) / (unsigned)g.splits) - 1 - first;
+    }
     // copy q of a stage into ring buffer `buf`: sub-stage by sub-stage, the L side first
     auto copy = [&](int stage, int buf, int q) __attribute__((always_inline)) {
         constexpr int HALF = LOADS / SUB / 2;
@@ -372,7 +499,7 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
             "s_nop 0\n\t"
             "global_load_lds_dwordx4 %0, %1"
             :
-            : "v"(voff + (unsigned)(stage * SUB + sub) * (kPiece * 2)), "s"(from[side] + i * hop[side]), "s"(to)
+            : "v"(voff + (unsigned)((first + stage) * SUB + sub) * (kPiece * 2)), "s"(from[side] + i * hop[side]), "s"(to)
             : "memory", "m0");
     };
 
@@ -434,7 +561,6 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
             group(at, yes, copying, nb, s + R, buf, decltype(at)::value + 1);
         });
     };
-    const int last = g.stages / SUB - 1;
     for (int s = 0; s < R && s <= last; s++)
 #pragma unroll
         for (int q = 0; q < LOADS; q++) copy(s, s, q);
@@ -462,125 +588,450 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
 #pragma unroll
         for (int z = 1; z < ACCS; z++) acc[i / F][i % F][0] += acc[i / F][i % F][z];
 
-    // ---- epilogue.  A lane holds column n32 of a block, rows 8 q + 4 half + 0..3 (q = 0..3).
-    // Transposed matrices (rows j) are read and written 16 bytes a lane: lanes n32 and n32 + 32
-    // hold neighbouring 8-byte pieces, of q = 2 t and 2 t + 1, and swap two of the four dwords.
+    if (SPLIT && g.splits > 1) {   // k_ortho_fold adds the parts up
+        f4* part = g.part + (((bt * (g.by_xcd ? gridDim.x / 8 : gridDim.x) + tile) * g.splits + blockIdx.z) * 4 + wave) * 256 + lane;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            part[64 * e] = f4{acc[0][0][0][4 * e], acc[0][0][0][4 * e + 1], acc[0][0][0][4 * e + 2], acc[0][0][0][4 * e + 3]};
+        return;
+    }
+
+    // ---- epilogue
     // The last step's values leave through LDS, a block column of the wavefront at a time: whole
     // rows of the result in either order.  Its operands are read (barrier).
     float (*out_stage)[32][33] = reinterpret_cast<float (*)[32][33]>(&lds[0][0][0] + wave * (F * 32 * 33 * 4));
     static_assert(sizeof(lds) >= 4 * F * 32 * 33 * 4, "the stage of the results fits into the ring");
     if (MODE == kLast) __syncthreads();
     const int end_i = g.w.mp, end_j = SYM ? g.w.mp : g.w.np;
-    const int quad = lane & 3;
-    const size_t mat_a = bt * g.w.mp * (size_t)g.w.ldm, mat_y = bt * g.w.np * (size_t)g.w.ldm;
-    // what is added to the product: X transposed (with its lo part), or A
-    const _Float16* addend = MODE == kGram ? nullptr : MODE == kPoly ? g.w.a + mat_a : g.w.y[g.cur] + mat_y;
-    constexpr bool HAS_LO = P == 3 || !SYM;
+    constexpr int BATCH = F == 4 ? 1 : F;   // blocks whose addends are loaded together; more do not
+                                            // fit beside 256 accumulators
 #pragma unroll
     for (int fj = 0; fj < F; fj++) {
-        const int jb = j0 + wj + 32 * fj, j = jb + n32;
+        const int jb = j0 + wj + 32 * fj;
         if (jb >= end_j) continue;   // whole blocks: the ends are multiples of 64
-        u4 add[F][2][2];   // [block][t][hi, lo]; the loads of BATCH blocks are in flight together
-        constexpr int BATCH = F == 4 ? (P == 3 ? 1 : 2) : F;   // more do not fit beside 256 accumulators
+        Addend add[F];
 #pragma unroll
         for (int f0 = 0; f0 < F; f0 += BATCH) {
-        if (MODE != kGram)
 #pragma unroll
-            for (int fi = f0; fi < f0 + BATCH; fi++) {
-                const int ib = i0 + wi + 32 * fi;
-                if (ib >= end_i) continue;
+            for (int fi = f0; fi < f0 + BATCH; fi++)
+                if (i0 + wi + 32 * fi < end_i) load_addend<P, MODE>(g, bt, i0 + wi + 32 * fi, jb, lane, add[fi]);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const _Float16* from_y = addend + at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
-                    add[fi][t][0] = *reinterpret_cast<const u4*>(from_y);
-                    if (P == 3) add[fi][t][1] = *reinterpret_cast<const u4*>(from_y + kLo);
-                    else if (HAS_LO) add[fi][t][1] = *reinterpret_cast<const u4*>(g.w.y_lo + mat_y + at<1>(j, g.w.ldm, ib + 16 * t) + 8 * half);
-                }
-            }
-#pragma unroll
-        for (int fi = f0; fi < f0 + BATCH; fi++) {
-            const int ib = i0 + wi + 32 * fi;
-            if (ib >= end_i) continue;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                if (MODE != kGram) {
-                    swap_halves(add[fi][t][0]);
-                    if (HAS_LO) swap_halves(add[fi][t][1]);
-                }
-                u4 hi_out, lo_out;   // dwords 0, 1: q = 2 t; 2, 3: q = 2 t + 1
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int q = 2 * t + u;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[e] = acc[fi][fj][0][4 * q + e];
-                        float x = 0.0f;
-                        if (MODE != kGram) {
-                            x = half_of(add[fi][t][0], 4 * u + e);
-                            if (HAS_LO) x += half_of(add[fi][t][1], 4 * u + e);
-                        }
-                        if (MODE == kGram) v[e] *= kScaleA / (kScaleX * kScaleX);
-                        else if (MODE == kPoly) v[e] = g.b * x + (g.c / kScaleA) * v[e];
-                        else v[e] = g.a * x + v[e] * (1.0f / kScaleA);
-                    }
-                    if (MODE == kLast) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            out_stage[fi][8 * q + 4 * half + e][n32] = v[e] * (1.0f / kScaleX);
-                        continue;
-                    }
-                    h4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        _Float16 p, r;
-                        split_hl(v[e], p, r);
-                        hi[e] = p; lo[e] = r;
-                    }
-                    const u2 hw = __builtin_bit_cast(u2, hi), lw = __builtin_bit_cast(u2, lo);
-                    hi_out[2 * u] = hw[0]; hi_out[2 * u + 1] = hw[1];
-                    lo_out[2 * u] = lw[0]; lo_out[2 * u + 1] = lw[1];
-                    // row-major: four lanes exchange their columns, one row of four entries each
-                    _Float16* to = MODE == kGram ? g.w.a + mat_a : MODE == kPoly ? g.w.b + mat_a
-                                                                                 : g.w.x + bt * g.w.mp * (size_t)g.w.ldn;
-                    to += at<P>(ib + 8 * q + 4 * half + quad, SYM ? g.w.ldm : g.w.ldn, jb + (n32 & 28));
-                    *reinterpret_cast<u2*>(to) = transpose_quad(hw, quad);
-                    if (P == 3) *reinterpret_cast<u2*>(to + kLo) = transpose_quad(lw, quad);
-                }
-                if (MODE == kLast) continue;
-                // a tile on the diagonal holds both halves itself, and has stored them
-                if (SYM && ti == tj) continue;
-                _Float16* to = SYM ? (MODE == kGram ? g.w.a : g.w.b) + mat_a : g.w.y[g.cur ^ 1] + mat_y;
-                to += at<P>(j, g.w.ldm, ib + 16 * t) + 8 * half;
-                swap_halves(hi_out);
-                *reinterpret_cast<u4*>(to) = hi_out;
-                if (HAS_LO) {
-                    swap_halves(lo_out);
-                    if (P == 3) *reinterpret_cast<u4*>(to + kLo) = lo_out;
-                    else *reinterpret_cast<u4*>(g.w.y_lo + mat_y + at<1>(j, g.w.ldm, ib + 16 * t) + 8 * half) = lo_out;
-                }
-            }
-        }
+            for (int fi = f0; fi < f0 + BATCH; fi++)
+                if (i0 + wi + 32 * fi < end_i)
+                    finish_block<P, MODE>(g, bt, acc[fi][fj][0], add[fi], i0 + wi + 32 * fi, jb, lane, SYM && ti == tj,
+                                          out_stage[MODE == kLast ? fi : 0]);
         }
         if (MODE == kLast) {
-            // rows of 32 values of the result, two a wavefront and instruction, eight in flight
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const OutArgs& o = g.out;
-            const int ib0 = i0 + wi;
 #pragma unroll 1
-            for (int b = 0; b < 2 * F; b++) {
-                const int ib = ib0 + 32 * (b >> 1), p0 = 16 * (b & 1) + half;
-                const int row0 = (o.tall ? jb : ib) + p0, col = (o.tall ? ib : jb) + n32;
-                if (ib >= end_i) break;
-                float v[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    v[k] = o.tall ? out_stage[b >> 1][n32][p0 + 2 * k] : out_stage[b >> 1][p0 + 2 * k][n32];
-                put_rows(o, bt * o.stride, row0, col, v);
-            }
+            for (int fi = 0; fi < F; fi++)
+                if (i0 + wi + 32 * fi < end_i) write_result(g.out, bt, i0 + wi + 32 * fi, jb, lane, out_stage[fi]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+
+// The parts of a tile of X X^T, added up in the order of the splits.  (A launch of its own: the
+// fences of a last-one-adds scheme inside the product cost 65 us a launch here, each writes back
+// an L2.)
+template <int P>
+__global__ __launch_bounds__(256) void k_ortho_fold(MulArgs g) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int ti, tj;
+    tile_of<true>(g, blockIdx.x, gridDim.x, ti, tj);
+    const size_t bt = blockIdx.y;
+    const f4* p = g.part + ((bt * gridDim.x + blockIdx.x) * g.splits * 4 + wave) * 256 + lane;
+    f16v sum;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sum[e] = 0.0f;
+#pragma unroll 4
+    for (int z = 0; z < g.splits; z++, p += 1024) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f4 v = p[64 * e];
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum[4 * e + k] += v[k];
+        }
+    }
+    Addend none;
+    finish_block<P, kGram>(g, bt, sum, none, ti * 64 + (wave & 1) * 32, tj * 64 + (wave >> 1) * 32, lane, ti == tj, nullptr);
+}
+
+// ---- A A and B X in one launch, for m up to 256 --------------------------------------------
+// There a step's three launches are 5 to 7 us each of which the matrix instructions are one: the
+// time is that of launches and first loads.  A workgroup makes the 32 rows of B that it needs
+// itself (m <= 256: at most as much work as its part of B X) and multiplies them with 128 columns
+// of X; B stays in LDS.  Stages of 64 values of A's rows, then of X transposed, go through one
+// ring without a break between the products.  MB = m / 64, so every count is known.
+// copies that may be in flight when stage s must have landed: those of the stages issued after it
+template <int S, int R, int LOADS_A, int LOADS_X>
+constexpr int flying(int s) {
+    int n = 0;
+    for (int t = s + 1; t < s + R - 1 && t < 2 * S; t++) n += t < S ? LOADS_A : LOADS_X;
+    return n;
+}
+template <int P, int MODE, int MB>
+__global__ __launch_bounds__(256) void k_ortho_pair(MulArgs g) {
+    constexpr int PL = P == 3 ? 2 : 1, S = MB * PL;       // stages of one product, 64 values each
+    constexpr int NB = (MB + 1) / 2;                      // blocks of B a wavefront makes at most
+    constexpr int LOADS_A = 2 * MB, LOADS_X = 4;          // copies a wavefront and stage
+    constexpr int ROWS = MB * 64 > 128 ? MB * 64 : 128;   // of a ring buffer
+    constexpr int R = MB > 3 ? 3 : 4;
+    constexpr int ACCS = P == 3 ? 3 : 2;
+    // own rows of A, then of B in their place: [32 values][32 rows][64 bytes], chunks swizzled as in
+    // the ring
+    __shared__ __align__(1024) unsigned char own[2 * S][32 * 64], ring[R][2][ROWS * 64];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+    const unsigned tile_i = g.by_xcd ? blockIdx.x / 8 : blockIdx.x;   // as in k_ortho_mul
+    const size_t bt = g.by_xcd ? blockIdx.z * 8 + blockIdx.x % 8 : blockIdx.z;
+    if (g.by_xcd && (int)bt >= g.by_xcd) return;
+    const int i0 = (int)tile_i * 32, j0 = (int)blockIdx.y * 128;
+    const size_t mat_a = bt * g.w.mp * (size_t)g.w.ldm, mat_y = bt * g.w.np * (size_t)g.w.ldm;
+    const unsigned voff = (unsigned)((lane >> 2) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16);
+    auto copy = [&](const _Float16* from, int stage, void* to) __attribute__((always_inline)) {
+        asm volatile(
+            "s_mov_b32 m0, %2\n\t"
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %0, %1"
+            :
+            : "v"(voff + (unsigned)stage * (kPiece * 2)), "s"(from), "s"((unsigned)(size_t)to)
+            : "memory", "m0");
+    };
+    const size_t row_of_pieces = (size_t)(2 * S) * kPiece;   // 16 rows of a matrix with ldm = 64 S
+    const _Float16* src_a = g.w.a + mat_a + wave * row_of_pieces;
+    const _Float16* src_x = g.w.y[g.cur] + mat_y + ((size_t)(j0 / 16) + wave) * row_of_pieces;
+    const _Float16* src_own = g.w.a + mat_a + (size_t)(i0 / 16) * row_of_pieces;
+    // stages 0 .. S - 1: A; S .. 2 S - 1: X transposed
+    auto copy_stage = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            unsigned char* to = ring[s % R][sub];
+            if (s < S) {
+#pragma unroll
+                for (int q = 0; q < MB; q++) copy(src_a + q * 4 * row_of_pieces, 2 * s + sub, to + (q * 4 + wave) * 1024);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2; q++) copy(src_x + q * 4 * row_of_pieces, 2 * (s - S) + sub, to + (q * 4 + wave) * 1024);
+            }
+        }
+    };
+    const int sw = (n32 >> 2) & 3;
+    auto operand = [&](const unsigned char* rows, int row0, int chunk) __attribute__((always_inline)) {
+        return *reinterpret_cast<const h8*>(rows + (row0 + n32) * 64 + ((chunk + half) ^ sw) * 16);
+    };
+    // one stage of L (32 own rows) times R (32 rows of the ring buffer) into acc
+    auto multiply = [&](const unsigned char* l, const unsigned char* r, int row0, f16v (&acc)[ACCS]) __attribute__((always_inline)) {
+        const h8 l0 = operand(l, 0, 0), l1 = operand(l, 0, 2), r0 = operand(r, row0, 0), r1 = operand(r, row0, 2);
+        acc[0] = mma(l0, r0, acc[0]);
+        if (P == 3) {   // hi and lo of 16 entries
+            acc[1] = mma(l0, r1, acc[1]);
+            acc[2] = mma(l1, r0, acc[2]);
+        } else {        // 32 entries
+            acc[1] = mma(l1, r1, acc[1]);
+        }
+    };
+    f16v acc[NB][ACCS];
+    auto clear = [](f16v (&a)[ACCS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int z = 0; z < ACCS; z++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) a[z][e] = 0.0f;
+    };
+    auto total = [](const f16v (&a)[ACCS]) __attribute__((always_inline)) {
+        f16v s = a[0];
+#pragma unroll
+        for (int z = 1; z < ACCS; z++) s += a[z];
+        return s;
+    };
+    // own rows of A first (oldest, so landed whenever a stage of the ring has)
+#pragma unroll
+    for (int q = 0; q < 4 * S; q += 4) {
+        const int piece = q + wave;   // of values 32 (piece / 2) .., rows 16 (piece % 2) ..
+        copy(src_own + (piece & 1) * row_of_pieces, piece >> 1, &own[piece >> 1][(piece & 1) * 1024]);
+    }
+#pragma unroll
+    for (int s = 0; s < R - 1; s++)
+        if (s < 2 * S) copy_stage(s);
+#pragma unroll
+    for (int b = 0; b < NB; b++) clear(acc[b]);
+    // Stage s has landed for this wavefront and, behind the barrier, for all; and all are done
+    // with stage s - 1, whose buffer takes stage s + R - 1.
+    auto turn = [&](auto at_s) __attribute__((always_inline)) {
+        constexpr int s = decltype(at_s)::value;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(flying<S, R, LOADS_A, LOADS_X>(s)) : "memory");
+        __syncthreads();
+        if (s + R - 1 < 2 * S) copy_stage(s + R - 1);
+    };
+    each(std::make_integer_sequence<int, S>{}, [&](auto at_s) __attribute__((always_inline)) {
+        constexpr int s = decltype(at_s)::value;
+        turn(at_s);
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                if (wave + 4 * b < 2 * MB) multiply(own[2 * s + sub], ring[s % R][sub], (wave + 4 * b) * 32, acc[b]);
+    });
+    // B = b A + c A A, own rows, in the form of an operand and in place of A: a wavefront replaces
+    // the columns that it alone still reads
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        if (wave + 4 * b >= 2 * MB) continue;
+        const int jb = (wave + 4 * b) * 32, quad = lane & 3;
+        const f16v sum = total(acc[b]);
+        // entry (row, k) of an operand: byte offset of its hi part
+        auto place = [&](int row, int k) {
+            const int chunk = P == 3 ? (k & 15) >> 3 : (k & 31) >> 3;
+            return (P == 3 ? k >> 4 : k >> 5) * (32 * 64) + row * 64 + ((chunk ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
+        };
+        auto place_lo = [&](int row, int k) {
+            return (k >> 4) * (32 * 64) + row * 64 + (((2 + ((k & 15) >> 3)) ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
+        };
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int row = 8 * (e >> 2) + 4 * half + (e & 3);
+            x[e] = (float)*reinterpret_cast<const _Float16*>(&own[0][0] + place(row, jb + n32));
+            if (P == 3) x[e] += (float)*reinterpret_cast<const _Float16*>(&own[0][0] + place_lo(row, jb + n32));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            h4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                _Float16 p, r;
+                split_hl(g.b * x[4 * q + e] + (g.c / kScaleA) * sum[4 * q + e], p, r);
+                hi[e] = p; lo[e] = r;
+            }
+            const int row = 8 * q + 4 * half + quad, k = jb + (n32 & 28);
+            *reinterpret_cast<u2*>(&own[0][0] + place(row, k)) = transpose_quad(__builtin_bit_cast(u2, hi), quad);
+            if (P == 3) *reinterpret_cast<u2*>(&own[0][0] + place_lo(row, k)) = transpose_quad(__builtin_bit_cast(u2, lo), quad);
+        }
+    }
+    clear(acc[0]);
+    each(std::make_integer_sequence<int, S>{}, [&](auto at_s) __attribute__((always_inline)) {
+        constexpr int s = S + decltype(at_s)::value;
+        turn(std::integral_constant<int, s>{});   // the first barrier also publishes B
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) multiply(own[2 * (s - S) + sub], ring[s % R][sub], wave * 32, acc[0]);
+    });
+    const int jb = j0 + 32 * wave;
+    static_assert(sizeof(ring) >= 4 * 32 * 33 * 4, "the stage of the results fits into the ring");
+    float (*out_stage)[33] = reinterpret_cast<float (*)[33]>(&ring[0][0][0] + wave * (32 * 33 * 4));
+    if (MODE == kLast) __syncthreads();
+    if (jb >= g.w.np) return;
+    Addend add;
+    load_addend<P, MODE>(g, bt, i0, jb, lane, add);
+    finish_block<P, MODE>(g, bt, total(acc[0]), add, i0, jb, lane, false, out_stage);
+    if (MODE == kLast) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        write_result(g.out, bt, i0, jb, lane, out_stage);
+    }
+}
+
+// ---- small matrices: everything in one workgroup -------------------------------------------
+// Where X, its transpose and A fit into LDS as operands (64 x 256 with P = 3, 128 x 128 with P = 1),
+// all steps run in one launch of one workgroup a matrix: the launches above cost 4 us each, the
+// work of one of them here is a fraction of one (all steps, fp32, launches / one workgroup each:
+// 1 x 32 x 32 50 / 20 us, 1 x 64 x 64 50 / 25, 1 x 64 x 256 57 / 44, 300 x 64 x 64 91 / 50,
+// 1000 x 32 x 128 238 / 94; bf16 1 x 128 x 128 50 / 41).  Bound by the chain of five barriers and
+// three products a step.  Operands are [32 values][rows][64 bytes] as in
+// k_ortho_pair.  A wavefront owns up to two 32 x 32 blocks and keeps their X in fp32 registers
+// (C layout: column n32, rows 8 q + 4 half + e), so the a X term needs no lo part.
+constexpr int kSmallWaves = 8, kSmallLds = 159 * 1024;
+struct SmallArgs {
+    InArgs in;
+    OutArgs out;
+    int mp, np;      // sides rounded up to 32
+    int steps;
+    float coef[3 * kMaxSteps];
+};
+template <int P>
+constexpr int small_bytes(int mp, int np) { return (2 * mp * np + mp * mp) * (P == 3 ? 4 : 2); }
+// byte offset of the hi part of entry (row, k) of an operand of `rows` rows; LO: of its lo part
+template <int P, bool LO = false>
+__device__ __forceinline__ int place_of(int rows, int row, int k) {
+    const int chunk = (P == 3 ? (k & 15) >> 3 : (k & 31) >> 3) + (LO ? 2 : 0);
+    return ((P == 3 ? k >> 4 : k >> 5) * rows + row) * 64 + ((chunk ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
+}
+// a block (ib, jb) into the operand whose rows are the block's rows, entry k its column
+template <int P>
+__device__ __forceinline__ void put_rows_of(unsigned char* m, int rows, int ib, int jb, int lane, const float (&v)[16]) {
+    const int n32 = lane & 31, half = lane >> 5, quad = lane & 3;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        h4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            _Float16 p, r;
+            split_hl(v[4 * q + e], p, r);
+            hi[e] = p; lo[e] = r;
+        }
+        const int row = ib + 8 * q + 4 * half + quad, k = jb + (n32 & 28);
+        *reinterpret_cast<u2*>(m + place_of<P>(rows, row, k)) = transpose_quad(__builtin_bit_cast(u2, hi), quad);
+        if (P == 3) *reinterpret_cast<u2*>(m + place_of<P, true>(rows, row, k)) = transpose_quad(__builtin_bit_cast(u2, lo), quad);
+    }
+}
+// ... and whose rows are the block's columns
+template <int P>
+__device__ __forceinline__ void put_columns_of(unsigned char* m, int rows, int ib, int jb, int lane, const float (&v)[16]) {
+    const int n32 = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        h4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            _Float16 p, r;
+            split_hl(v[4 * q + e], p, r);
+            hi[e] = p; lo[e] = r;
+        }
+        const int k = ib + 8 * q + 4 * half;
+        *reinterpret_cast<h4*>(m + place_of<P>(rows, jb + n32, k)) = hi;
+        if (P == 3) *reinterpret_cast<h4*>(m + place_of<P, true>(rows, jb + n32, k)) = lo;
+    }
+}
+// block (ib, jb) of L R^T over `count` times 32 values
+template <int P>
+__device__ __forceinline__ f16v product_of(const unsigned char* l, int lrows, int ib, const unsigned char* r, int rrows, int jb,
+                                           int count, int lane) {
+    const int n32 = lane & 31, half = lane >> 5, sw = (n32 >> 2) & 3;
+    const unsigned char *lp = l + (ib + n32) * 64, *rp = r + (jb + n32) * 64;
+    const int c0 = (half ^ sw) * 16, c1 = ((2 + half) ^ sw) * 16;
+    f16v acc[3];
+#pragma unroll
+    for (int z = 0; z < 3; z++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[z][e] = 0.0f;
+#pragma unroll 2
+    for (int s = 0; s < count; s++, lp += lrows * 64, rp += rrows * 64) {
+        const h8 l0 = *reinterpret_cast<const h8*>(lp + c0), l1 = *reinterpret_cast<const h8*>(lp + c1);
+        const h8 r0 = *reinterpret_cast<const h8*>(rp + c0), r1 = *reinterpret_cast<const h8*>(rp + c1);
+        acc[0] = mma(l0, r0, acc[0]);
+        if (P == 3) {
+            acc[1] = mma(l0, r1, acc[1]);
+            acc[2] = mma(l1, r0, acc[2]);
+        } else {
+            acc[1] = mma(l1, r1, acc[1]);
+        }
+    }
+    acc[0] += acc[1];
+    if (P == 3) acc[0] += acc[2];
+    return acc[0];
+}
+template <int P>
+__global__ __launch_bounds__(64 * kSmallWaves) void k_ortho_small(SmallArgs g) {
+    __shared__ __align__(1024) unsigned char lds[kSmallLds];
+    __shared__ double ws[kSmallWaves];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n32 = lane & 31, half = lane >> 5;
+    const int mp = g.mp, np = g.np, nbi = mp / 32, blocks = nbi * (np / 32), blocks_a = nbi * nbi;
+    const int values = P == 3 ? 16 : 32;    // entries in 32 values
+    unsigned char* const x_op = lds;                                    // rows of X
+    unsigned char* const y_op = x_op + (size_t)mp * np * (P == 3 ? 4 : 2);   // its columns
+    unsigned char* const a_op = y_op + (size_t)mp * np * (P == 3 ? 4 : 2);   // A, then B
+    const InArgs& in = g.in;
+    const OutArgs& o = g.out;
+    const size_t bt = blockIdx.x;
+    float x[2][16];
+    double sum = 0.0;
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        const int id = wave + kSmallWaves * b, ib = id % nbi * 32, jb = id / nbi * 32;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int i = ib + 8 * (e >> 2) + 4 * half + (e & 3), j = jb + n32;
+            const int row = o.tall ? j : i, col = o.tall ? i : j;
+            x[b][e] = 0.0f;
+            if (id < blocks && row < in.rows && col < in.cols) {
+                const size_t at_g = bt * in.stride + (size_t)row * in.ld + col;
+                float u = load_any(in.g, in.dtype, at_g);
+                if (in.mom) {
+                    const float m = in.beta * in.mom[at_g] + u;
+                    in.mom[at_g] = m;
+                    u = in.nesterov ? u + in.beta * m : m;
+                }
+                if (in.g_clear) in.g_clear[at_g] = 0.0f;
+                x[b][e] = u;
+                sum += (double)u * (double)u;
+            }
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) ws[wave] = sum;
+    __syncthreads();
+    double norm = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSmallWaves; w++) norm += ws[w];
+    norm = sqrt(norm) + (double)in.eps;
+    const double inv = norm == 0.0 ? 0.0 : (double)kScaleX / norm;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[b][e] = (float)((double)x[b][e] * inv);
+#pragma unroll 1
+    for (int s = 0; s < g.steps; s++) {
+        const float ca = g.coef[3 * s], cb = g.coef[3 * s + 1], cc = g.coef[3 * s + 2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int id = wave + kSmallWaves * b;
+            if (id >= blocks) continue;
+            put_rows_of<P>(x_op, mp, id % nbi * 32, id / nbi * 32, lane, x[b]);
+            put_columns_of<P>(y_op, np, id % nbi * 32, id / nbi * 32, lane, x[b]);
+        }
+        __syncthreads();
+        float a[2][16];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int id = wave + kSmallWaves * b, ib = id % nbi * 32, jb = id / nbi * 32;
+            if (id >= blocks_a) continue;
+            const f16v p = product_of<P>(x_op, mp, ib, x_op, mp, jb, np / values, lane);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                a[b][e] = p[e] * (kScaleA / (kScaleX * kScaleX));
+                // one product: b A takes the A that A A is made of, so that their errors go together
+                if (P == 1) a[b][e] = (float)(_Float16)a[b][e];
+            }
+            put_rows_of<P>(a_op, mp, ib, jb, lane, a[b]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int id = wave + kSmallWaves * b, ib = id % nbi * 32, jb = id / nbi * 32;
+            if (id >= blocks_a) continue;
+            const f16v p = product_of<P>(a_op, mp, ib, a_op, mp, jb, mp / values, lane);
+#pragma unroll
+            for (int e = 0; e < 16; e++) a[b][e] = cb * a[b][e] + (cc / kScaleA) * p[e];
+        }
+        __syncthreads();   // A is read
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int id = wave + kSmallWaves * b;
+            if (id < blocks_a) put_rows_of<P>(a_op, mp, id % nbi * 32, id / nbi * 32, lane, a[b]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int id = wave + kSmallWaves * b;
+            if (id >= blocks) continue;
+            const f16v p = product_of<P>(a_op, mp, id % nbi * 32, y_op, np, id / nbi * 32, mp / values, lane);
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[b][e] = ca * x[b][e] + p[e] * (1.0f / kScaleA);
+        }
+        __syncthreads();   // X transposed and B are read
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        const int id = wave + kSmallWaves * b, ib = id % nbi * 32, jb = id / nbi * 32;
+        if (id >= blocks) continue;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int i = ib + 8 * (e >> 2) + 4 * half + (e & 3), j = jb + n32;
+            const int row = o.tall ? j : i, col = o.tall ? i : j;
+            if (row < o.rows && col < o.cols) put_out(o, bt * o.stride + (size_t)row * o.ld + col, x[b][e] * (1.0f / kScaleX));
         }
     }
 }
@@ -603,44 +1054,12 @@ __global__ __launch_bounds__(256) void k_ortho_copy(Work w, OutArgs t) {
 // ---- plan ------------------------------------------------------------------------------
 struct Plan {
     int mp, np, ldm, ldn, groups;
-    size_t part, x, y, y_lo, ab, total;   // bytes
+    int splits;   // of X X^T
+    bool small;   // k_ortho_small
+    size_t part, x, y, y_lo, ab, split_part, total;   // bytes
 };
 constexpr int kOverhang = 256 - 64;
 size_t round_up(size_t v, size_t q) { return (v + q - 1) / q * q; }
-Plan make_plan(int batch, int rows, int cols, int products) {
-    Plan p{};
-    const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    p.mp = (int)round_up(m, 64);
-    p.np = (int)round_up(n, 64);
-    const int planes = products == 3 ? 2 : 1;
-    p.ldm = p.mp * planes;
-    p.ldn = p.np * planes;
-    const size_t h = sizeof(_Float16);
-    // a wavefront of the first pass takes two or more pieces of 256 columns
-    const int64_t units = (int64_t)rows * ((cols + 255) / 256);
-    p.groups = (int)(units / 8 < 1 ? 1 : units / 8 > kMaxNormGroups ? kMaxNormGroups : units / 8);
-    p.part = round_up((size_t)batch * p.groups * sizeof(double), 256);
-    // A tile that hangs over the last row of a batch reads up to kOverhang rows behind it: into
-    // the next matrix or this slack.  What it reads there reaches only rows that are not stored.
-    p.x = round_up(((size_t)batch * p.mp + kOverhang) * p.ldn * h, 256);
-    p.y = round_up(((size_t)batch * p.np + kOverhang) * p.ldm * h, 256);
-    p.y_lo = products == 1 ? round_up((size_t)batch * p.np * p.ldm * h, 256) : 0;
-    p.ab = round_up(((size_t)batch * p.mp + kOverhang) * p.ldm * h, 256);
-    p.total = p.part + p.x + 2 * p.y + p.y_lo + 2 * p.ab;
-    return p;
-}
-
-template <int P, int MODE, int F, int SUB, int R>
-void run_mul(MulArgs g, int batch, hipStream_t st) {
-    constexpr int T = 64 * F;
-    constexpr bool SYM = MODE == kGram || MODE == kPoly;
-    g.tiles_i = (g.w.mp + T - 1) / T;
-    const int tiles_j = (g.w.np + T - 1) / T;
-    const int tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
-    g.row_len = SYM ? g.tiles_i + 1 : g.tiles_i;
-    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
-    hipLaunchKernelGGL((k_ortho_mul<P, MODE, F, SUB, R>), dim3(tiles, batch), dim3(256), 0, st, g);
-}
 // Tile size of a product: rounds of 256 workgroups (one a CU) times what a tile costs relative to
 // a 64 x 64 one.  A tile twice as wide does four times the work in 2.1 times the time: it reads
 // half as much from L2 and LDS an operation.  Measured at 4096 x 4096, P = 1: B X on tiles of
@@ -659,6 +1078,65 @@ int tile_for(bool sym, int rows, int cols, int batch) {
     }
     return best;
 }
+Plan make_plan(int batch, int rows, int cols, int products) {
+    Plan p{};
+    const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    p.mp = (int)round_up(m, 32);
+    p.np = (int)round_up(n, 32);
+    p.small = p.mp <= 1024 && p.np <= 1024 && p.mp * p.np <= 2 * kSmallWaves * 1024 &&
+              (products == 3 ? small_bytes<3>(p.mp, p.np) : small_bytes<1>(p.mp, p.np)) <= kSmallLds;
+    if (p.small) return p;   // no workspace
+    p.mp = (int)round_up(m, 64);
+    p.np = (int)round_up(n, 64);
+    const int planes = products == 3 ? 2 : 1;
+    p.ldm = p.mp * planes;
+    p.ldn = p.np * planes;
+    const size_t h = sizeof(_Float16);
+    // a wavefront of the first pass takes two or more pieces of 256 columns
+    const int64_t units = (int64_t)rows * ((cols + 255) / 256);
+    p.groups = (int)(units / 8 < 1 ? 1 : units / 8 > kMaxNormGroups ? kMaxNormGroups : units / 8);
+    p.part = round_up((size_t)batch * p.groups * sizeof(double), 256);
+    // A tile that hangs over the last row of a batch reads up to kOverhang rows behind it: into
+    // the next matrix or this slack.  What it reads there reaches only rows that are not stored.
+    p.x = round_up(((size_t)batch * p.mp + kOverhang) * p.ldn * h, 256);
+    p.y = round_up(((size_t)batch * p.np + kOverhang) * p.ldm * h, 256);
+    p.y_lo = products == 1 ? round_up((size_t)batch * p.np * p.ldm * h, 256) : 0;
+    p.ab = round_up(((size_t)batch * p.mp + kOverhang) * p.ldm * h, 256);
+    // X X^T of few small tiles with many stages: the stages shared out until about two workgroups a
+    // CU run, none with less than 16 stages of 64 values (all steps, fp32, unsplit / 8 / 16 / 32 stages:
+    // 1 x 64 x 2048: 101 / 75 / 78 / 88 us, 1 x 250 x 4000: 200 / 139 / 136 / 149,
+    // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000 bf16: 80 / 86 / 80 / 80)
+    p.splits = 1;
+    if (tile_for(true, p.mp, p.mp, batch) == 1) {
+        const int64_t nt = p.mp / 64, tiles = nt * (nt + 1) / 2 * batch;
+        const int64_t room = 512 / tiles, most = p.ldn / 64 / 16;
+        const int64_t splits = room < most ? room : most;
+        p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
+        if (p.splits > 1) p.split_part = (size_t)tiles * p.splits * 64 * 64 * sizeof(float);
+    }
+    p.total = p.part + p.x + 2 * p.y + p.y_lo + 2 * p.ab + p.split_part;
+    return p;
+}
+
+// An XCD takes whole matrices while their tiles find a CU each there (32 of them): its L2 fetches
+// its own matrices only (9 x 256 x 256 fp32, all steps: 93 us instead of 109).
+bool one_xcd_each(int batch, int64_t tiles) { return batch >= 8 && tiles * ((batch + 7) / 8) <= 32; }
+
+template <int P, int MODE, int F, int SUB, int R>
+void run_mul(MulArgs g, int batch, hipStream_t st) {
+    constexpr int T = 64 * F;
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    g.tiles_i = (g.w.mp + T - 1) / T;
+    const int tiles_j = (g.w.np + T - 1) / T;
+    const int tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
+    g.row_len = SYM ? g.tiles_i + 1 : 4 * tiles_j;
+    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
+    const int per_xcd = (batch + 7) / 8;
+    g.by_xcd = one_xcd_each(batch, tiles) ? batch : 0;
+    hipLaunchKernelGGL((k_ortho_mul<P, MODE, F, SUB, R>), dim3(g.by_xcd ? 8 * tiles : tiles, g.by_xcd ? per_xcd : batch, MODE == kGram && F == 1 ? g.splits : 1), dim3(256),
+                       0, st, g);
+    if (MODE == kGram && F == 1 && g.splits > 1) hipLaunchKernelGGL(k_ortho_fold<P>, dim3(tiles, batch), dim3(256), 0, st, g);
+}
 // Ring buffers: three to four stages in flight where they fit into 160 KiB (with two, a stage of
 // small tiles is over before the copies of the next have landed: 42 instead of 19 us above); tiles
 // of 128 with P = 1 run faster as two workgroups a CU of two stages each.
@@ -673,9 +1151,38 @@ void run_mul(const MulArgs& g, int batch, hipStream_t st) {
     }
 }
 
+// The pair kernel reads all of A in every workgroup: worth it up to 128 KiB of A (m = 128 with
+// P = 3, 256 with P = 1) and while one or two rounds of workgroups do.  All five steps, with it and
+// without: 1 x 128 x 512 fp32 68 / 80 us, 1 x 192 x 800 fp32 95 / 95, 1 x 256 x 843 fp32 114 / 104,
+// the same in bf16 78 / 84.
+template <int P>
+bool use_pair(const Work& w, int batch) {
+    return w.mp <= (P == 3 ? 128 : 256) && (int64_t)(w.mp / 32) * ((w.np + 127) / 128) * batch <= 512;
+}
+template <int P, int MODE>
+void run_pair(MulArgs g, int batch, hipStream_t st) {
+    const int ti = g.w.mp / 32, tj = (g.w.np + 127) / 128, per_xcd = (batch + 7) / 8;
+    g.by_xcd = one_xcd_each(batch, ti * tj) ? batch : 0;
+    const dim3 grid(g.by_xcd ? 8 * ti : ti, tj, g.by_xcd ? per_xcd : batch), block(256);
+    switch (g.w.mp / 64) {
+        case 1: hipLaunchKernelGGL((k_ortho_pair<P, MODE, 1>), grid, block, 0, st, g); break;
+        case 2: hipLaunchKernelGGL((k_ortho_pair<P, MODE, 2>), grid, block, 0, st, g); break;
+        case 3: if constexpr (P == 1) hipLaunchKernelGGL((k_ortho_pair<P, MODE, 3>), grid, block, 0, st, g); break;
+        default: if constexpr (P == 1) hipLaunchKernelGGL((k_ortho_pair<P, MODE, 4>), grid, block, 0, st, g); break;
+    }
+}
+
 template <int P>
 int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const float* coef, const Plan& p, char* work,
             hipStream_t st) {
+    if (p.small) {
+        SmallArgs g{};
+        g.in = in; g.out = out; g.mp = p.mp; g.np = p.np; g.steps = steps;
+        for (int i = 0; i < 3 * steps; i++) g.coef[i] = coef[i];
+        hipLaunchKernelGGL(k_ortho_small<P>, dim3(batch), dim3(64 * kSmallWaves), 0, st, g);
+        CFP_HIP_TRY(hipGetLastError());
+        return 0;
+    }
     Work w{};
     InArgs a = in;
     a.part = (double*)work;             work += p.part;
@@ -688,7 +1195,8 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
     w.y[1] = (_Float16*)work;           work += p.y;
     w.y_lo = P == 1 ? (_Float16*)work : nullptr; work += p.y_lo;
     w.a = (_Float16*)work;              work += p.ab;
-    w.b = (_Float16*)work;
+    w.b = (_Float16*)work;              work += p.ab;
+    f4* split_part = (f4*)work;
     w.mp = p.mp; w.np = p.np; w.ldm = p.ldm; w.ldn = p.ldn;
     const int tall = out.tall;
     hipLaunchKernelGGL(k_ortho_norm, dim3(p.groups, batch), dim3(256), 0, st, a);
@@ -706,7 +1214,13 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
         g.a = coef[3 * s]; g.b = coef[3 * s + 1]; g.c = coef[3 * s + 2];
         g.out = out;
         g.l = g.r = w.x; g.ldl = g.ldr = p.ldn; g.l_batch = g.r_batch = xb; g.stages = p.ldn / 32;
+        g.splits = p.splits; g.part = split_part;
         run_mul<P, kGram>(g, batch, st);
+        if (use_pair<P>(w, batch)) {
+            if (s + 1 < steps) run_pair<P, kStep>(g, batch, st);
+            else run_pair<P, kLast>(g, batch, st);
+            continue;
+        }
         g.l = g.r = w.a; g.ldl = g.ldr = p.ldm; g.l_batch = g.r_batch = ab; g.stages = p.ldm / 32;
         run_mul<P, kPoly>(g, batch, st);
         g.l = w.b; g.r = w.y[g.cur]; g.ldl = g.ldr = p.ldm; g.l_batch = ab; g.r_batch = yb; g.stages = p.ldm / 32;
@@ -768,7 +1282,7 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
                 "cfp_orthogonalize: input or output not aligned to its type");
     const int p = products ? products : dtype == CFP_BF16 ? 1 : 3;
     const Plan plan = make_plan(batch, rows, cols, p);
-    CFP_REQUIRE(d_work && work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(d_work) & 255u) == 0,
+    CFP_REQUIRE(plan.total == 0 || (d_work && work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(d_work) & 255u) == 0),
                 "cfp_orthogonalize: needs a 256-byte aligned workspace of %zu bytes (got %zu)", plan.total, work_bytes);
     float c[3 * kMaxSteps];
     fill_coef(coefs, steps, c);
@@ -797,7 +1311,7 @@ int muon_update(const MuonArgs& u, hipStream_t st) {
                 "cfp_muon_update: arrays not aligned to fp32");
     const int p = u.products ? u.products : 3;
     const Plan plan = make_plan(u.batch, u.rows, u.cols, p);
-    CFP_REQUIRE(u.work && u.work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(u.work) & 255u) == 0,
+    CFP_REQUIRE(plan.total == 0 || (u.work && u.work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(u.work) & 255u) == 0),
                 "cfp_muon_update: needs a 256-byte aligned workspace of %zu bytes (got %zu)", plan.total, u.work_bytes);
     float c[3 * kMaxSteps];
     fill_coef(u.coefs, u.steps, c);

@@ -458,7 +458,8 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
  * fp32, the norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes all
  * of it NaN.
  * d_work: cfp_orthogonalize_workspace(batch, rows, cols, products) bytes (products 1 or 3),
- * 256-byte aligned; calls that may overlap need one each. */
+ * 256-byte aligned (may be NULL where that is 0: matrices that fit into one workgroup); calls that
+ * may overlap need one each. */
 size_t cfp_orthogonalize_workspace(int batch, int rows, int cols, int products);
 int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stride, int batch,
                       int rows, int cols, int steps, const float* coefs, float eps, int products,

@@ -27,7 +27,8 @@ def _muon(lib, w=P, g=P, m=P, ld=64, stride=64 * 64, batch=1, rows=64, cols=64, 
     (dict(out=None), "NULL"), (dict(ld=63), "strides"), (dict(ldo=63), "strides"),
     (dict(batch=2, stride=64 * 64 - 1), "overlap"), (dict(batch=2, so=0), "overlap"),
     (dict(g=C.c_void_p(0x10002)), "aligned"), (dict(dtype=1, out=C.c_void_p(0x10001)), "aligned"),
-    (dict(work=None), "workspace"), (dict(nbytes=1000), "workspace"), (dict(work=C.c_void_p(0x10010)), "workspace"),
+    (dict(work=None, rows=300), "workspace"), (dict(nbytes=1000, rows=300), "workspace"),
+    (dict(work=C.c_void_p(0x10010), rows=300), "workspace"),
 ])
 def test_orthogonalize_refuses(pkg, kw, word):
     lib = pkg.lib()
@@ -38,7 +39,7 @@ def test_orthogonalize_refuses(pkg, kw, word):
 @pytest.mark.parametrize("kw,word", [
     (dict(w=None), "NULL"), (dict(g=None), "NULL"), (dict(m=None), "NULL"), (dict(ld=10), "stride"),
     (dict(batch=3, stride=9), "overlap"), (dict(steps=99), "steps"), (dict(products=5), "products"),
-    (dict(m=C.c_void_p(0x10002)), "aligned"), (dict(work=None), "workspace"), (dict(nbytes=1), "workspace"),
+    (dict(m=C.c_void_p(0x10002)), "aligned"), (dict(work=None, rows=300), "workspace"), (dict(nbytes=1, rows=300), "workspace"),
     (dict(rows=1 << 17), "rows"), (dict(eps=-0.5), "eps"),
 ])
 def test_muon_refuses(pkg, kw, word):
@@ -55,6 +56,8 @@ def test_no_matrices_is_no_work(pkg):
 def test_workspace_sizes(pkg):
     ws = pkg.lib().cfp_orthogonalize_workspace
     assert ws(0, 64, 64, 1) == 0 and ws(1, 0, 64, 1) == 0 and ws(1, 64, 64, 2) == 0 and ws(1, 64, 1 << 17, 1) == 0
+    assert ws(9, 64, 256, 3) == 0 and ws(1, 128, 128, 1) == 0     # one workgroup, no workspace
+    assert ws(1, 128, 128, 3) > 0 and ws(1, 64, 300, 3) > 0 and ws(1, 128, 160, 1) > 0
     one, three = ws(1, 1000, 3000, 1), ws(1, 1000, 3000, 3)
     # three matrices of the gradient's size and two of the shorter side squared, at least
     assert one >= 2 * (3 * 1000 * 3000 + 2 * 1000 * 1000) and three > one
