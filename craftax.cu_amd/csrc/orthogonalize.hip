@@ -263,7 +263,9 @@ struct MulArgs {
     size_t l_batch, r_batch; // values a matrix
     int stages;              // of 32 values; even
     int tiles_i;
-    unsigned row_len;        // tiles of a pair of rows (symmetric products) or of a band of four
+    int tiles;               // of one matrix
+    int runs;                // an XCD takes a run of tiles
+    unsigned row_len;        // tiles of a pair of rows (symmetric products), of a column, or of a band
     uint64_t row_inv;        // ceil(2^32 / row_len)
     int by_xcd;              // 0, or the matrices of the batch where one XCD takes each
     Work w;
@@ -276,6 +278,13 @@ struct MulArgs {
 };
 __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Loads the arguments that lead to a workgroup's first copies at once: left to the branches that
+// use them they are five loads one after the other (0.25 us a launch).
+__device__ __forceinline__ void load_args(const MulArgs& g) {
+    asm volatile("" ::"s"(g.l), "s"(g.r), "s"(g.ldl), "s"(g.ldr), "s"(g.l_batch), "s"(g.r_batch), "s"(g.stages), "s"(g.tiles_i),
+                 "s"(g.tiles), "s"(g.runs), "s"(g.row_len), "s"(g.row_inv), "s"(g.by_xcd), "s"(g.splits));
 }
 
 // Waits until at most min(later, MOST) * LOADS of this wave's copies are in flight.  Copies are
@@ -425,14 +434,12 @@ __device__ __forceinline__ void each(std::integer_sequence<int, I...>, Fn&& f) {
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-// Tile t of `total`.  In scalar arithmetic throughout (addresses of copies are scalar operands):
+// Tile of number t.  In scalar arithmetic throughout (addresses of copies are scalar operands):
 // t / d as t * ceil(2^32 / d) / 2^32, exact while t * d < 2^32.
 template <bool SYM>
-__device__ __forceinline__ void tile_of(const MulArgs& g, unsigned t, unsigned total, int& ti, int& tj) {
-    // Workgroups go to the eight XCDs in turn; an XCD takes a run of tiles, which share panels in its
-    // L2 (2048 x 8192 bf16, all steps: 992 us instead of 1040).
-    if (!g.by_xcd) {
-        const unsigned x = t % 8, q = total / 8, r = total % 8;
+__device__ __forceinline__ void tile_of(const MulArgs& g, unsigned t, int& ti, int& tj) {
+    if (g.runs) {
+        const unsigned x = t % 8, q = (unsigned)g.tiles / 8, r = (unsigned)g.tiles % 8;
         t = x * q + (x < r ? x : r) + t / 8;
     }
     if (SYM) {
@@ -441,8 +448,11 @@ __device__ __forceinline__ void tile_of(const MulArgs& g, unsigned t, unsigned t
         const int n = g.tiles_i, r = (int)row, c = (int)col;
         ti = c < n - r ? r : n - 1 - r;
         tj = c < n - r ? r + c : c - 1;
-    } else {
-        // bands of four tile rows, column by column
+    } else if (!g.runs) {   // column by column
+        const unsigned col = (unsigned)((t * g.row_inv) >> 32);
+        ti = (int)(t - col * g.row_len);
+        tj = (int)col;
+    } else {                // bands of four tile rows, each column by column
         const unsigned band = (unsigned)((t * g.row_inv) >> 32), rest = t - band * g.row_len;
         const unsigned rows = (unsigned)g.tiles_i - 4 * band;   // of the last band: 1 to 4
         const unsigned col = rows >= 4 ? rest >> 2 : rows == 3 ? (rest * 43691u) >> 17 : rows == 2 ? rest >> 1 : rest;
@@ -470,12 +480,13 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
     constexpr int NM = (P == 3 ? 3 : 1) * F * F, NR = 2 * PL * F;
     __shared__ __align__(1024) unsigned char lds[R][SUB][2 * T * 64];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+    load_args(g);
     // by_xcd: blockIdx.y and the residue of blockIdx.x (the XCD) name the matrix
     const unsigned tile = g.by_xcd ? blockIdx.x / 8 : blockIdx.x;
     const size_t bt = g.by_xcd ? blockIdx.y * 8 + blockIdx.x % 8 : blockIdx.y;
     if (g.by_xcd && (int)bt >= g.by_xcd) return;
     int ti, tj;
-    tile_of<SYM>(g, tile, g.by_xcd ? gridDim.x / 8 : gridDim.x, ti, tj);
+    tile_of<SYM>(g, tile, ti, tj);
     const int i0 = ti * T, j0 = tj * T;
     // this wave's pieces of stage 0: F of the L side, F of the R side
     const _Float16* from[2] = {g.l + bt * g.l_batch + (size_t)(i0 / 16 + wave) * (g.ldl >> 5) * kPiece,
@@ -589,7 +600,7 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
         for (int z = 1; z < ACCS; z++) acc[i / F][i % F][0] += acc[i / F][i % F][z];
 
     if (SPLIT && g.splits > 1) {   // k_ortho_fold adds the parts up
-        f4* part = g.part + (((bt * (g.by_xcd ? gridDim.x / 8 : gridDim.x) + tile) * g.splits + blockIdx.z) * 4 + wave) * 256 + lane;
+        f4* part = g.part + (((bt * g.tiles + tile) * g.splits + blockIdx.z) * 4 + wave) * 256 + lane;
 #pragma unroll
         for (int e = 0; e < 4; e++)
             part[64 * e] = f4{acc[0][0][0][4 * e], acc[0][0][0][4 * e + 1], acc[0][0][0][4 * e + 2], acc[0][0][0][4 * e + 3]};
@@ -640,9 +651,9 @@ template <int P>
 __global__ __launch_bounds__(256) void k_ortho_fold(MulArgs g) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int ti, tj;
-    tile_of<true>(g, blockIdx.x, gridDim.x, ti, tj);
+    tile_of<true>(g, blockIdx.x, ti, tj);
     const size_t bt = blockIdx.y;
-    const f4* p = g.part + ((bt * gridDim.x + blockIdx.x) * g.splits * 4 + wave) * 256 + lane;
+    const f4* p = g.part + ((bt * g.tiles + blockIdx.x) * g.splits * 4 + wave) * 256 + lane;
     f16v sum;
 #pragma unroll
     for (int e = 0; e < 16; e++) sum[e] = 0.0f;
@@ -684,6 +695,7 @@ __global__ __launch_bounds__(256) void k_ortho_pair(MulArgs g) {
     // the ring
     __shared__ __align__(1024) unsigned char own[2 * S][32 * 64], ring[R][2][ROWS * 64];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+    asm volatile("" ::"s"(g.w.a), "s"(g.w.y[0]), "s"(g.w.y[1]), "s"(g.cur), "s"(g.w.mp), "s"(g.w.np), "s"(g.w.ldm), "s"(g.by_xcd));
     const unsigned tile_i = g.by_xcd ? blockIdx.x / 8 : blockIdx.x;   // as in k_ortho_mul
     const size_t bt = g.by_xcd ? blockIdx.z * 8 + blockIdx.x % 8 : blockIdx.z;
     if (g.by_xcd && (int)bt >= g.by_xcd) return;
@@ -1105,12 +1117,13 @@ Plan make_plan(int batch, int rows, int cols, int products) {
     // X X^T of few small tiles with many stages: the stages shared out until about two workgroups a
     // CU run, none with less than 16 stages of 64 values (all steps, fp32, unsplit / 8 / 16 / 32 stages:
     // 1 x 64 x 2048: 101 / 75 / 78 / 88 us, 1 x 250 x 4000: 200 / 139 / 136 / 149,
-    // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000 bf16: 80 / 86 / 80 / 80)
+    // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000 bf16: 80 / 86 / 80 / 80).  Two workgroups
+    // a tile on half of the CUs gain nothing (1 x 1000 x 2731 bf16: 200 us unsplit, 219 split).
     p.splits = 1;
     if (tile_for(true, p.mp, p.mp, batch) == 1) {
         const int64_t nt = p.mp / 64, tiles = nt * (nt + 1) / 2 * batch;
         const int64_t room = 512 / tiles, most = p.ldn / 64 / 16;
-        const int64_t splits = room < most ? room : most;
+        const int64_t splits = tiles > 128 ? 1 : room < most ? room : most;
         p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
         if (p.splits > 1) p.split_part = (size_t)tiles * p.splits * 64 * 64 * sizeof(float);
     }
@@ -1128,11 +1141,17 @@ void run_mul(MulArgs g, int batch, hipStream_t st) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly;
     g.tiles_i = (g.w.mp + T - 1) / T;
     const int tiles_j = (g.w.np + T - 1) / T;
-    const int tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
-    g.row_len = SYM ? g.tiles_i + 1 : 4 * tiles_j;
-    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
+    const int tiles = g.tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
     const int per_xcd = (batch + 7) / 8;
     g.by_xcd = one_xcd_each(batch, tiles) ? batch : 0;
+    // Workgroups go to the eight XCDs in turn.  Where the CUs take more than one each, an XCD takes a
+    // run of tiles of neighbouring rows and columns, which share panels in its L2; one tile a CU is
+    // faster in plain order, where an XCD keeps to one row's panel (all steps, runs / plain order:
+    // 2048 x 8192 bf16 998 / 1030 us, 1000 x 2731 fp32 292 / 302; 2 x 500 x 1000 fp32 160 / 135,
+    // 700 x 700 fp32 138 / 124).
+    g.runs = !g.by_xcd && (int64_t)tiles * F * batch > 256;
+    g.row_len = SYM ? g.tiles_i + 1 : g.runs ? 4 * tiles_j : g.tiles_i;
+    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
     hipLaunchKernelGGL((k_ortho_mul<P, MODE, F, SUB, R>), dim3(g.by_xcd ? 8 * tiles : tiles, g.by_xcd ? per_xcd : batch, MODE == kGram && F == 1 ? g.splits : 1), dim3(256),
                        0, st, g);
     if (MODE == kGram && F == 1 && g.splits > 1) hipLaunchKernelGGL(k_ortho_fold<P>, dim3(tiles, batch), dim3(256), 0, st, g);
