@@ -286,6 +286,7 @@ __device__ __forceinline__ void put_rows(const OutArgs& o, size_t base, int row0
 
 // ---- the product C[i][j] = sum_k L[i][k] R[j][k] and what is made of it ---------------
 enum { kGram, kPoly, kStep, kLast };
+constexpr int kBlockWaves = 8;   // of k_ortho_block
 struct MulArgs {
     const _Float16* l;
     const _Float16* r;
@@ -671,6 +672,83 @@ __global__ __launch_bounds__(256) void k_ortho_mul(MulArgs g) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
+    }
+}
+
+// ---- the same products where they leave most CUs idle ----------------------------------------
+// A workgroup makes one 32 x 32 block and its wavefronts share out the K axis: every wavefront
+// reads operands of its own, from L2 straight into registers, the parts meet in LDS and are added
+// in the order of the wavefronts.  Bound by the round trips to memory, one for every four stages of
+// a wavefront, and by the launch.  All steps, fp32, with k_ortho_mul / this kernel: 256 x 843
+// 104 / 97 us, 500 x 1000 130 / 119, 16 x 128 x 512 78 / 73.
+template <int P, int MODE>
+__global__ __launch_bounds__(64 * kBlockWaves) void k_ortho_block(MulArgs g) {
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    __shared__ f4 part[kBlockWaves][4][64];
+    __shared__ float out_stage[MODE == kLast ? 32 : 1][33];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n32 = lane & 31, half = lane >> 5;
+    load_args(g);
+    const unsigned tile = g.by_xcd ? blockIdx.x / 8 : blockIdx.x;   // as in k_ortho_mul
+    const size_t bt = g.by_xcd ? blockIdx.y * 8 + blockIdx.x % 8 : blockIdx.y;
+    if (g.by_xcd && (int)bt >= g.by_xcd) return;
+    int ti, tj;
+    tile_of<SYM>(g, tile, ti, tj);
+    const int first = g.stages * wave / kBlockWaves, count = g.stages * (wave + 1) / kBlockWaves - first;
+    // piece of rows n32 / 16, row n32 % 16 of it, entries 8 half and up: a lane's first 16 bytes
+    const _Float16* l = g.l + bt * g.l_batch + ((size_t)(2 * ti + (n32 >> 4)) * (g.ldl >> 5) + first) * kPiece + (n32 & 15) * 32 + 8 * half;
+    const _Float16* r = g.r + bt * g.r_batch + ((size_t)(2 * tj + (n32 >> 4)) * (g.ldr >> 5) + first) * kPiece + (n32 & 15) * 32 + 8 * half;
+    f16v acc[3];
+#pragma unroll
+    for (int z = 0; z < 3; z++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[z][e] = 0.0f;
+    Addend add;
+    if (wave == 0) load_addend<P, MODE>(g, bt, ti * 32, tj * 32, lane, add);
+    constexpr int U = 4;   // stages whose operands are loaded together
+    auto stages = [&](auto many) __attribute__((always_inline)) {
+        constexpr int N = decltype(many)::value;
+        h8 l0[N], l1[N], r0[N], r1[N];
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            l0[u] = *reinterpret_cast<const h8*>(l + u * kPiece); l1[u] = *reinterpret_cast<const h8*>(l + u * kPiece + 16);
+            r0[u] = *reinterpret_cast<const h8*>(r + u * kPiece); r1[u] = *reinterpret_cast<const h8*>(r + u * kPiece + 16);
+        }
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            acc[0] = mma(l0[u], r0[u], acc[0]);
+            if (P == 3) {
+                acc[1] = mma(l0[u], r1[u], acc[1]);
+                acc[2] = mma(l1[u], r0[u], acc[2]);
+            } else {
+                acc[1] = mma(l1[u], r1[u], acc[1]);
+            }
+        }
+        l += N * kPiece; r += N * kPiece;
+    };
+    int s = 0;
+    for (; s + U <= count; s += U) stages(std::integral_constant<int, U>{});
+    if (count - s >= 2) { stages(std::integral_constant<int, 2>{}); s += 2; }
+    if (count - s >= 1) stages(std::integral_constant<int, 1>{});
+    acc[0] += acc[1];
+    if (P == 3) acc[0] += acc[2];
+    if (wave > 0)
+#pragma unroll
+        for (int e = 0; e < 4; e++) part[wave][e][lane] = f4{acc[0][4 * e], acc[0][4 * e + 1], acc[0][4 * e + 2], acc[0][4 * e + 3]};
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < kBlockWaves; w++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f4 v = part[w][e][lane];
+#pragma unroll
+            for (int k = 0; k < 4; k++) acc[0][4 * e + k] += v[k];
+        }
+    finish_block<P, MODE>(g, bt, acc[0], add, ti * 32, tj * 32, lane, ti == tj, out_stage);
+    if (MODE == kLast) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        write_result(g.out, bt, ti * 32, tj * 32, lane, out_stage);
     }
 }
 
@@ -1120,6 +1198,13 @@ int tile_for(bool sym, int rows, int cols, int batch) {
     }
     return best;
 }
+// k_ortho_block while its blocks find a CU each (two or four: 700 x 700 fp32, all steps, 130 us
+// instead of 120) and a wavefront's share of the K axis is short (of 126 stages: 250 x 2000 fp32
+// 124 us, split over workgroups 118; of 63: bf16 91 us, split 99)
+bool in_blocks(bool sym, int rows, int cols, int batch, int stages) {
+    const int64_t ti = rows / 32, tj = cols / 32;
+    return (sym ? ti * (ti + 1) / 2 : ti * tj) * batch <= 256 && stages <= 100;
+}
 Plan make_plan(int batch, int rows, int cols, int products) {
     Plan p{};
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
@@ -1150,7 +1235,7 @@ Plan make_plan(int batch, int rows, int cols, int products) {
     // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000 bf16: 80 / 86 / 80 / 80).  Two workgroups
     // a tile on half of the CUs gain nothing (1 x 1000 x 2731 bf16: 200 us unsplit, 219 split).
     p.splits = 1;
-    if (tile_for(true, p.mp, p.mp, batch) == 1) {
+    if (tile_for(true, p.mp, p.mp, batch) == 1 && !in_blocks(true, p.mp, p.mp, batch, p.ldn / 32)) {
         const int64_t nt = p.mp / 64, tiles = nt * (nt + 1) / 2 * batch;
         const int64_t room = 512 / tiles, most = p.ldn / 64 / 16;
         const int64_t splits = tiles > 128 ? 1 : room < most ? room : most;
@@ -1186,12 +1271,23 @@ void run_mul(MulArgs g, int batch, hipStream_t st) {
                        0, st, g);
     if (MODE == kGram && F == 1 && g.splits > 1) hipLaunchKernelGGL(k_ortho_fold<P>, dim3(tiles, batch), dim3(256), 0, st, g);
 }
+template <int P, int MODE>
+void run_block(MulArgs g, int batch, hipStream_t st) {
+    constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    g.tiles_i = g.w.mp / 32;
+    const int tiles_j = g.w.np / 32, tiles = g.tiles = SYM ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * tiles_j;
+    g.by_xcd = one_xcd_each(batch, tiles) ? batch : 0;
+    g.row_len = SYM ? g.tiles_i + 1 : g.tiles_i;
+    g.row_inv = (((uint64_t)1 << 32) + g.row_len - 1) / g.row_len;
+    hipLaunchKernelGGL((k_ortho_block<P, MODE>), dim3(g.by_xcd ? 8 * tiles : tiles, g.by_xcd ? (batch + 7) / 8 : batch), dim3(64 * kBlockWaves), 0, st, g);
+}
 // Ring buffers: three to four stages in flight where they fit into 160 KiB (with two, a stage of
 // small tiles is over before the copies of the next have landed: 42 instead of 19 us above); tiles
 // of 128 with P = 1 run faster as two workgroups a CU of two stages each.
 template <int P, int MODE>
 void run_mul(const MulArgs& g, int batch, hipStream_t st) {
     constexpr bool SYM = MODE == kGram || MODE == kPoly;
+    if (in_blocks(SYM, g.w.mp, SYM ? g.w.mp : g.w.np, batch, g.stages)) { run_block<P, MODE>(g, batch, st); return; }
     switch (tile_for(SYM, g.w.mp, SYM ? g.w.mp : g.w.np, batch)) {
         case 4: run_mul<P, MODE, 4, P == 1 ? 1 : 2, P == 1 ? 4 : 2>(g, batch, st); break;
         case 3: run_mul<P, MODE, 3, 2, 3>(g, batch, st); break;

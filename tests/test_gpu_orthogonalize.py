@@ -75,7 +75,8 @@ def off(got, want):
 SHAPES = [(1, 1, 1), (1, 1, 7), (1, 9, 1), (2, 3, 5), (1, 31, 33), (3, 64, 64), (1, 65, 64), (1, 63, 130), (9, 256, 256),
           (1, 843, 256), (1, 256, 843), (2, 300, 1000), (1, 1000, 2731), (1, 2050, 700), (1, 40, 5000),
           (1, 128, 128), (2, 192, 700), (40, 250, 256), (3, 130, 3000), (1, 64, 9000), (1, 500, 4500),
-          (300, 32, 32), (2, 64, 256), (3, 256, 61), (2, 97, 100), (1, 20, 500), (1, 128, 126)]
+          (300, 32, 32), (2, 64, 256), (3, 256, 61), (2, 97, 100), (1, 20, 500), (1, 128, 126),
+          (1, 500, 1000), (4, 256, 843)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
