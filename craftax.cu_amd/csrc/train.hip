@@ -1,5 +1,5 @@
 // On-device PPO update: rollout slabs, windowed recompute backward, GAE,
-// Adam.  Host-side mirror of the reference's CuTrain layer
+// Adam or Muon.  Host-side mirror of the reference's CuTrain layer
 // (craftax_full.cu:12637-13480).  The streaming kernels (reverse MinGRU sweep, head
 // gradients, GAE, Adam) live in ppo_kernels.hip, the GEMMs behind the seam of
 // gemm.hip / gemm_x9.hip; here: the window loop, the two-stream schedule, graph
@@ -864,7 +864,7 @@ int cfp_train_muon(cfp_trainer* tr, void* stream) {
 }
 
 // cu_train_body without its collect (craftax_full.cu:13348-13366): per epoch the loss
-// sums start at zero, then every minibatch's backward is followed by its Adam step.
+// sums start at zero, then every minibatch's backward is followed by its optimiser step.
 static int train_body(cfp_trainer* tr, void* stream) {
     for (int e = 0; e < tr->cfg.epochs; e++) {
         int rc = cfp_train_zero_loss(tr, stream);

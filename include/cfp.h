@@ -623,7 +623,8 @@ int cfp_train_muon(cfp_trainer* tr, void* stream);
 /* cu_train_body without its collect + cu_train_update (craftax_full.cu:13348-13406):
  * one PPO iteration over the stored rollout (slabs, adv/ret and the advantage
  * statistics already in place): epochs x (loss sums reset, minibatches x
- * (cfp_train_backward of the m-th contiguous env slice, cfp_train_adam)), then a
+ * (cfp_train_backward of the m-th contiguous env slice, cfp_train_adam or, with
+ * CFP_OPT_MUON, cfp_train_muon)), then a
  * synchronisation of the stream, as in the reference.  use_graph != 0 is the
  * reference's graph mode: the first call captures the iteration once on `stream`
  * (on a stream of the trainer's own when `stream` is NULL, which cannot be
