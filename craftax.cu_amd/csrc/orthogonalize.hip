@@ -1393,6 +1393,18 @@ void fill_coef(const float* coefs, int steps, float (&c)[3 * kMaxSteps]) {
     for (int i = 0; i < 3 * steps; i++) c[i] = coefs ? coefs[i] : kQuintic[i % 3];
 }
 size_t type_bytes(int dtype) { return dtype == CFP_F32 ? 4 : 2; }
+// Whether two batches of matrices share no entry: address ranges apart, or the same strides with
+// columns side by side.
+bool apart(const void* a, int64_t ld_a, int64_t stride_a, const void* b, int64_t ld_b, int64_t stride_b, int batch, int rows,
+           int cols, size_t bytes) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t a1 = a0 + (((batch - 1) * stride_a) + (rows - 1) * ld_a + cols) * bytes;
+    const uintptr_t b1 = b0 + (((batch - 1) * stride_b) + (rows - 1) * ld_b + cols) * bytes;
+    if (a1 <= b0 || b1 <= a0) return true;
+    if (ld_a != ld_b || ld_a < 1 || (batch > 1 && (stride_a != stride_b || stride_a % ld_a))) return false;
+    const int64_t d = (int64_t)((a0 > b0 ? a0 - b0 : b0 - a0) / bytes) % ld_a;
+    return d >= cols && d <= ld_a - cols;
+}
 
 }  // namespace
 }  // namespace cfp
@@ -1425,6 +1437,9 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
     const unsigned am = (unsigned)type_bytes(dtype) - 1u;
     CFP_REQUIRE(((reinterpret_cast<uintptr_t>(d_g) | reinterpret_cast<uintptr_t>(d_out)) & am) == 0,
                 "cfp_orthogonalize: input or output not aligned to its type");
+    CFP_REQUIRE((d_g == d_out && (ld == ld_out || rows == 1) && (batch_stride == out_batch_stride || batch == 1)) ||
+                    apart(d_g, ld, batch_stride, d_out, ld_out, out_batch_stride, batch, rows, cols, type_bytes(dtype)),
+                "cfp_orthogonalize: the output may replace the input, with the same strides, but not overlap it otherwise");
     const int p = products ? products : dtype == CFP_BF16 ? 1 : 3;
     const Plan plan = make_plan(batch, rows, cols, p);
     CFP_REQUIRE(plan.total == 0 || (d_work && work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(d_work) & 255u) == 0),
@@ -1458,6 +1473,11 @@ int muon_update(const MuonArgs& u, hipStream_t st) {
     const Plan plan = make_plan(u.batch, u.rows, u.cols, p);
     CFP_REQUIRE(plan.total == 0 || (u.work && u.work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(u.work) & 255u) == 0),
                 "cfp_muon_update: needs a 256-byte aligned workspace of %zu bytes (got %zu)", plan.total, u.work_bytes);
+    for (const float* pair : {u.g, u.mom})
+        CFP_REQUIRE(apart(u.w, u.ld, u.stride, pair, u.ld, u.stride, u.batch, u.rows, u.cols, 4),
+                    "cfp_muon_update: weight, gradient and momentum must not overlap");
+    CFP_REQUIRE(apart(u.g, u.ld, u.stride, u.mom, u.ld, u.stride, u.batch, u.rows, u.cols, 4),
+                "cfp_muon_update: weight, gradient and momentum must not overlap");
     float c[3 * kMaxSteps];
     fill_coef(u.coefs, u.steps, c);
     InArgs in{};

@@ -451,7 +451,7 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
  *   A = X X^T,  B = b A + c A A,  X = a X + B X      (on the shorter side of G)
  * d_g and d_out: `batch` matrices rows x cols (1..65536 each) of element type `dtype`, row
  * strides ld / ld_out and matrix strides batch_stride / out_batch_stride in elements (any for a
- * batch of one); d_out may be d_g.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315) for
+ * batch of one); d_out may be d_g with the same strides, any other overlap is an error.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315) for
  * every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
  * products: 1 = one fp16 matrix product per product (2e-3 of the result's norm from the 64-bit
  * result), 3 = three (1e-6, as fp32), 0 = by type: 1 for bf16, 3 for fp32 and fp16.  Sums are
@@ -470,7 +470,8 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
  *   m = momentum m + g,   u = g + momentum m (nesterov != 0) or m,   O = the above of u,
  *   w = w (1 - lr weight_decay) - lr scale O
  * lr is multiplied by *d_lr when that is not NULL (device memory: a captured step follows it).
- * scale 0 = sqrt(max(1, rows / cols)).  products 0 = 3.  Workspace as above. */
+ * scale 0 = sqrt(max(1, rows / cols)).  products 0 = 3.  Workspace as above.  w, g and m must not
+ * overlap. */
 int cfp_muon_update(float* d_w, const float* d_g, float* d_momentum, int64_t ld,
                     int64_t batch_stride, int batch, int rows, int cols, const float* d_lr, float lr,
                     float momentum, int nesterov, float weight_decay, float scale, int steps,

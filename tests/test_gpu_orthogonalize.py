@@ -242,6 +242,34 @@ def test_same_call_same_bits_on_any_stream_and_from_a_graph(pkg, cuda):
             assert (w - w2).abs().max().item() <= 2.0 ** -20
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(300, 40, 60), (5, 64, 256), (2, 500, 330)])
+def test_small_matrices_from_a_graph_in_place_and_side_by_side(pkg, cuda, dtype, shape):
+    """One workgroup a matrix and many: captured and replayed, in place, columns beside the input's."""
+    torch = _torch()
+    pol = pkg.policy
+    batch, rows, cols = shape
+    g = gradient(cuda, *shape, dtype, seed=11)
+    wide = torch.full((batch, rows, 2 * cols + 1), 3.0, dtype=g.dtype, device=cuda)
+    wide[:, :, 1:cols + 1].copy_(g)
+    want = pol.orthogonalize(g)
+    pol.orthogonalize(wide[:, :, 1:cols + 1], out=wide[:, :, cols + 1:])
+    assert torch.equal(wide[:, :, cols + 1:], want) and torch.equal(wide[:, :, 1:cols + 1], g) and wide[:, :, 0].eq(3).all()
+    buf = g.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pol.orthogonalize(buf, out=buf)
+    for rep in range(4):
+        g = gradient(cuda, *shape, dtype, seed=30 + rep)
+        buf.copy_(g)
+        eager = pol.orthogonalize(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(buf, eager)
+        assert off(buf, reference(g)) <= tolerance(dtype, 1 if dtype == "bf16" else 3, shape)
+
+
 def test_two_calls_at_once(pkg, cuda):
     """Two streams, each call with a workspace of its own."""
     torch = _torch()

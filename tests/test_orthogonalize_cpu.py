@@ -48,6 +48,25 @@ def test_muon_refuses(pkg, kw, word):
     assert word in lib.cfp_last_error().decode()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=C.c_void_p(0x10004)), dict(ldo=65), dict(batch=2, so=64 * 65), dict(out=C.c_void_p(0x10000 + 64 * 64 * 4 - 4)),
+    dict(ld=127, ldo=127, out=C.c_void_p(0x10000 + 64 * 4)), dict(ld=128, ldo=128, out=C.c_void_p(0x10000 + 63 * 4)),
+    dict(ld=128, ldo=128, out=C.c_void_p(0x10000 + 65 * 4)),
+])
+def test_orthogonalize_refuses_an_output_across_the_input(pkg, kw):
+    assert _ortho(pkg.lib(), **{**dict(rows=64, cols=64), **kw}) != 0
+    assert b"overlap" in pkg.lib().cfp_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(g=C.c_void_p(0x10000 + BIG)), dict(m=C.c_void_p(0x10000 + BIG)), dict(w=C.c_void_p(0x10000 + BIG)),
+    dict(g=C.c_void_p(0x10000 + 64 * 64 * 4), m=C.c_void_p(0x10000 + 64 * 64 * 8 - 4)),
+])
+def test_muon_refuses_arrays_across_each_other(pkg, kw):
+    assert _muon(pkg.lib(), **kw) != 0
+    assert b"overlap" in pkg.lib().cfp_last_error()
+
+
 def test_no_matrices_is_no_work(pkg):
     assert _ortho(pkg.lib(), batch=0, g=None, out=None, work=None, nbytes=0) == 0
     assert _muon(pkg.lib(), batch=0, w=None, g=None, m=None, work=None, nbytes=0) == 0
