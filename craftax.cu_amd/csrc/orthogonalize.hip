@@ -60,7 +60,7 @@ struct InArgs {
     int dtype;
     int64_t ld, stride;
     int rows, cols;
-    int vec;             // rows start on four-element boundaries
+    int vec;             // rows start and end on four-element boundaries
     float* mom;          // or null; same ld and stride as g
     float beta;
     int nesterov;
@@ -73,19 +73,44 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, size_t i) {
     return dtype == CFP_F32 ? ((const float*)p)[i]
                             : dtype == CFP_BF16 ? (float)((const __bf16*)p)[i] : (float)((const _Float16*)p)[i];
 }
-// four consecutive entries, the first `count` of which exist
-__device__ __forceinline__ f4 load_four(const void* p, int dtype, size_t i, int count, bool vec) {
-    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (vec && count >= 4) {
-        if (dtype == CFP_F32) return *reinterpret_cast<const f4*>((const float*)p + i);
-        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-        if (dtype == CFP_BF16) return __builtin_convertvector(*reinterpret_cast<const b4*>((const __bf16*)p + i), f4);
-        return __builtin_convertvector(*reinterpret_cast<const h4*>((const _Float16*)p + i), f4);
+// N pieces of four entries, at i[k] + e * HOP: entry e of piece k exists when e < count[k].  Without
+// a branch between the loads, so that all are in flight together: entries that do not exist are read
+// from `any` (an entry that does) and replaced by zero.  Vectors (HOP = 1) exist whole or not at all.
+template <int N, int HOP>
+__device__ __forceinline__ void load_pieces(const void* p, int dtype, bool vec, const size_t (&i)[N], const int (&count)[N],
+                                            size_t any, f4 (&v)[N]) {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    if (vec && dtype == CFP_F32) {
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = *reinterpret_cast<const f4*>((const float*)p + (count[k] > 0 ? i[k] : any));
+    } else if (vec) {
+        u2 raw[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) raw[k] = *reinterpret_cast<const u2*>((const _Float16*)p + (count[k] > 0 ? i[k] : any));
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            v[k] = dtype == CFP_BF16 ? __builtin_convertvector(__builtin_bit_cast(b4, raw[k]), f4)
+                                     : __builtin_convertvector(__builtin_bit_cast(h4, raw[k]), f4);
+    } else if (dtype == CFP_F32) {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[k][e] = ((const float*)p)[e < count[k] ? i[k] + e * HOP : any];
+    } else {
+        _Float16 raw[N][4];
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) raw[k][e] = ((const _Float16*)p)[e < count[k] ? i[k] + e * HOP : any];
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[k][e] = dtype == CFP_BF16 ? (float)__builtin_bit_cast(__bf16, raw[k][e]) : (float)raw[k][e];
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (e < count) v[e] = load_any(p, dtype, i + e);
-    return v;
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[k][e] = e < count[k] ? v[k][e] : 0.0f;
 }
 __device__ __forceinline__ void store_four(float* p, size_t i, int count, bool vec, const f4& v) {
     if (vec && count >= 4) { *reinterpret_cast<f4*>(p + i) = v; return; }
@@ -103,7 +128,8 @@ __global__ __launch_bounds__(256) void k_ortho_norm(InArgs a) {
     const int lane = threadIdx.x & 63;
     double s = 0.0;
     // two pieces at a time, all loads before the first use (with the momentum of a 1000 x 2731 fp32
-    // matrix, 33 MB: 10 us; one at a time, four neighbouring entries a lane: 15)
+    // matrix, 33 MB: 8 us; one at a time, four neighbouring entries a lane and a branch around each
+    // load: 15)
     const unsigned hop = (unsigned)a.groups * 4;
     for (unsigned u0 = blockIdx.x * 4 + (threadIdx.x >> 6); u0 < units; u0 += 2 * hop) {
         f4 v[2], m[2];
@@ -116,18 +142,12 @@ __global__ __launch_bounds__(256) void k_ortho_norm(InArgs a) {
             const int c = (int)(u - r * segs) * 256 + (a.vec ? 4 : 1) * lane;
             count[k] = u < units ? a.vec ? a.cols - c : (a.cols - c + 63) >> 6 : 0;
             at_g[k] = base + (size_t)r * a.ld + c;
-            v[k] = m[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (a.vec) {
-                v[k] = load_four(a.g, a.dtype, at_g[k], count[k], true);
-                if (a.mom) m[k] = load_four(a.mom, CFP_F32, at_g[k], count[k], true);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (e < count[k]) {
-                        v[k][e] = load_any(a.g, a.dtype, at_g[k] + 64 * e);
-                        if (a.mom) m[k][e] = a.mom[at_g[k] + 64 * e];
-                    }
-            }
+        }
+        if (a.vec) load_pieces<2, 1>(a.g, a.dtype, true, at_g, count, base, v);
+        else load_pieces<2, 64>(a.g, a.dtype, false, at_g, count, base, v);
+        if (a.mom) {
+            if (a.vec) load_pieces<2, 1>(a.mom, CFP_F32, true, at_g, count, base, m);
+            else load_pieces<2, 64>(a.mom, CFP_F32, false, at_g, count, base, m);
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
@@ -175,14 +195,20 @@ __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) 
     const int r0 = (int)blockIdx.y * 64, c0 = (int)blockIdx.x * 64;
     const int x4 = 4 * (threadIdx.x & 15), y = threadIdx.x >> 4;
     f4 u[4];
+    size_t from[4];
+    int have[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const int r = r0 + 16 * k + y, c = c0 + x4, count = r < a.rows ? a.cols - c : 0;
-        u[k] = load_four(a.g, a.dtype, base + (size_t)r * a.ld + c, count, a.vec);
-        if (a.mom) {
-            const f4 m = load_four(a.mom, CFP_F32, base + (size_t)r * a.ld + c, count, a.vec);
-            u[k] = a.nesterov ? u[k] + a.beta * m : m;
-        }
+        const int r = r0 + 16 * k + y, c = c0 + x4;
+        have[k] = r < a.rows ? a.cols - c : 0;
+        from[k] = base + (size_t)r * a.ld + c;
+    }
+    load_pieces<4, 1>(a.g, a.dtype, a.vec, from, have, base, u);
+    if (a.mom) {
+        f4 m[4];
+        load_pieces<4, 1>(a.mom, CFP_F32, a.vec, from, have, base, m);
+#pragma unroll
+        for (int k = 0; k < 4; k++) u[k] = a.nesterov ? u[k] + a.beta * m[k] : m[k];
     }
     double s = 0.0;
     for (int i = threadIdx.x; i < a.groups; i += 256) s += a.part[(size_t)bt * a.groups + i];
@@ -211,8 +237,8 @@ __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) 
     };
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const int r = r0 + 16 * k + y, c = c0 + x4, count = r < a.rows ? a.cols - c : 0;
-        if (a.g_clear) store_four(a.g_clear, base + (size_t)r * a.ld + c, count, a.vec, f4{0.0f, 0.0f, 0.0f, 0.0f});
+        const int r = r0 + 16 * k + y, c = c0 + x4;
+        if (a.g_clear) store_four(a.g_clear, from[k], have[k], a.vec, f4{0.0f, 0.0f, 0.0f, 0.0f});
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -1332,7 +1358,7 @@ int run_all(const InArgs& in, const OutArgs& out, int batch, int steps, const fl
     InArgs a = in;
     a.part = (double*)work;             work += p.part;
     a.groups = p.groups;
-    a.vec = a.ld % 4 == 0 && a.stride % 4 == 0 &&
+    a.vec = a.cols % 4 == 0 && a.ld % 4 == 0 && a.stride % 4 == 0 &&
             (reinterpret_cast<uintptr_t>(a.g) & (a.dtype == CFP_F32 ? 15u : 7u)) == 0 &&
             (reinterpret_cast<uintptr_t>(a.mom) & 15u) == 0;
     w.x = (_Float16*)work;              work += p.x;
