@@ -270,6 +270,21 @@ def test_small_matrices_from_a_graph_in_place_and_side_by_side(pkg, cuda, dtype,
         assert off(buf, reference(g)) <= tolerance(dtype, 1 if dtype == "bf16" else 3, shape)
 
 
+def test_arrays_packed_matrix_by_matrix(pkg, cuda):
+    """Weights, gradients and momentum of a layer behind each other, and rows taken in turn."""
+    torch = _torch()
+    for shape in ((4, 3, 50, 70), (4, 50, 3, 70)):
+        packed = torch.full(shape, 2.0, device=cuda)
+        at = (lambda k: packed[:, k]) if shape[1] == 3 else (lambda k: packed[:, :, k])
+        w, g, m = (at(k) for k in range(3))
+        for i, t in enumerate((w, g, m)):
+            t.copy_(gradient(cuda, 4, 50, 70, seed=40 + i))
+        w2, g2, m2 = (t.contiguous().clone() for t in (w, g, m))
+        pkg.policy.muon_update(w, g, m, 0.1)
+        pkg.policy.muon_update(w2, g2, m2, 0.1)
+        assert torch.equal(w, w2) and torch.equal(g, g2) and torch.equal(m, m2)
+
+
 def test_two_calls_at_once(pkg, cuda):
     """Two streams, each call with a workspace of its own."""
     torch = _torch()
