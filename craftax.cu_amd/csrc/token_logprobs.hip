@@ -14,6 +14,7 @@
 // m + ln s has lost the bits of ln s.  All sums are fp32 per lane (at most a few hundred terms
 // each, in [0, 1]) and joined in a tree of fixed shape: the same call gives the same bits.
 #include <float.h>
+#include <limits.h>
 
 #include "cfp_internal.h"
 
@@ -119,6 +120,18 @@ template <int WIDTH>
 __device__ __forceinline__ float max_lanes(float v) {
     return reduce_lanes<WIDTH>(v, [](float a, float b) { return fmaxf(a, b); });
 }
+template <int WIDTH>
+__device__ __forceinline__ int min_lanes(int v) {
+    v = min(v, (int)xor_lane<1>((unsigned)v));
+    v = min(v, (int)xor_lane<2>((unsigned)v));
+    v = min(v, (int)xor_lane<4>((unsigned)v));
+    v = min(v, (int)xor_lane<8>((unsigned)v));
+    if (WIDTH == 64) {
+        v = min(v, (int)xor_lane<16>((unsigned)v));
+        v = min(v, (int)xor_lane<32>((unsigned)v));
+    }
+    return v;
+}
 __device__ __forceinline__ void join_lanes(Sums& a) {
     raise_max(a, max_lanes<64>(a.m));
     a.s = sum_lanes<64>(a.s);
@@ -145,7 +158,6 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
     return (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
            (unsigned)__builtin_amdgcn_readlane((int)k, lane);
 }
-__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 template <int D>
 __device__ __forceinline__ uint64_t xor_key(uint64_t k) {
     return (uint64_t)xor_lane<D>((unsigned)(k >> 32)) << 32 | xor_lane<D>((unsigned)k);
@@ -234,6 +246,18 @@ struct Best {
         if (waiting > 0) merge(top);
     }
 };
+
+// the same for 16-bit types and indices below 2^16
+template <typename T>
+__device__ __forceinline__ unsigned short_key(float v, int i) {
+    const unsigned u = __builtin_bit_cast(unsigned short, (T)(v + 0.0f));   // exact: v came from a T
+    return (u ^ (u & 0x8000u ? 0xffffu : 0x8000u)) << 16 | (unsigned)(0xffff - i);
+}
+template <typename T>
+__device__ __forceinline__ float short_value(unsigned key) {
+    const unsigned h = key >> 16;
+    return to_f32(__builtin_bit_cast(T, (unsigned short)(h & 0x8000u ? h ^ 0x8000u : h ^ 0xffffu)));
+}
 
 struct LpArgs {
     const void* x;
@@ -353,31 +377,68 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
         z.s = sum_lanes<L>(z.s);
         z.u = sum_lanes<L>(z.u);
         if (live && sub == 0) write_row(a, row, z, tok, xt);
+        if (a.top == 0) continue;
+        // Alternatives: the maximum of the row, then the lowest index that holds it, `top` times; lane
+        // k (then k - L) keeps number k, and all are written together.  16-bit entries and their index
+        // make one 32-bit key (rows have at most 1024 of them): 262 144 x 43 fp16 with 20 alternatives
+        // take 85 us, 150 with value and index apart, as fp32 has them (111).
+        constexpr int SLOTS = kMaxTop > L ? kMaxTop / L : 1;
+        if constexpr (sizeof(T) == 2) {
+            unsigned key[Q][N], kept[SLOTS] = {};
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int j = 0; j < N; j++) key[q][j] = v[q][j] > -INFINITY ? short_key<T>(v[q][j], first[q] + j) : 0u;
+            for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
+                unsigned best = 0;
+#pragma unroll
+                for (int q = 0; q < Q; q++)
+#pragma unroll
+                    for (int j = 0; j < N; j++) best = max(best, key[q][j]);
+                best = max(best, xor_lane<1>(best));
+                best = max(best, xor_lane<2>(best));
+                best = max(best, xor_lane<4>(best));
+                best = max(best, xor_lane<8>(best));
+                if (L == 64) {
+                    best = max(best, xor_lane<16>(best));
+                    best = max(best, xor_lane<32>(best));
+                }
+#pragma unroll
+                for (int q = 0; q < Q; q++)
+#pragma unroll
+                    for (int j = 0; j < N; j++) key[q][j] = key[q][j] == best ? 0u : key[q][j];
+#pragma unroll
+                for (int t = 0; t < SLOTS; t++) kept[t] = k == t * L + sub ? best : kept[t];
+            }
+#pragma unroll
+            for (int t = 0; t < SLOTS; t++)
+                if (live && t * L + sub < a.top)
+                    write_top(a, row, z, t * L + sub, kept[t] ? key_of(short_value<T>(kept[t]), 0xffff - (int)(kept[t] & 0xffffu)) : 0);
+            continue;
+        }
+        uint64_t kept[SLOTS] = {};
         for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
             float bv = -INFINITY;
-            int bi = -1;
+            int bi = INT_MAX;
 #pragma unroll
             for (int q = 0; q < Q; q++)
 #pragma unroll
                 for (int j = 0; j < N; j++)   // ascending index: ties keep the first
                     if (v[q][j] > bv) { bv = v[q][j]; bi = first[q] + j; }
-            uint64_t best = bi >= 0 ? key_of(bv, bi) : 0;
-            best = larger(best, xor_key<1>(best));
-            best = larger(best, xor_key<2>(best));
-            best = larger(best, xor_key<4>(best));
-            best = larger(best, xor_key<8>(best));
-            if (L == 64) {
-                best = larger(best, xor_key<16>(best));
-                best = larger(best, xor_key<32>(best));
-            }
-            bi = key_index(best);
+            const float m = max_lanes<L>(bv);
+            bi = min_lanes<L>(bv == m ? bi : INT_MAX);
 #pragma unroll
             for (int q = 0; q < Q; q++)
 #pragma unroll
                 for (int j = 0; j < N; j++)
                     if (first[q] + j == bi) v[q][j] = -INFINITY;
-            if (live && sub == 0) write_top(a, row, z, k, best);
+#pragma unroll
+            for (int t = 0; t < SLOTS; t++)
+                if (k == t * L + sub) kept[t] = bi == INT_MAX ? 0 : key_of(m, bi);
         }
+#pragma unroll
+        for (int t = 0; t < SLOTS; t++)
+            if (live && t * L + sub < a.top) write_top(a, row, z, t * L + sub, kept[t]);
     }
 }
 
@@ -870,15 +931,17 @@ struct LpPlan {
     int kind;     // 0 short, 1 a wavefront a row, 2 a workgroup a split
     int splits, chunk;
 };
-// Rows of up to 2 KiB sit in the registers of 16 or 64 lanes (1 KiB from four alternatives on, 512
-// bytes from nine on: finding them one by one costs 70 to 110 instructions each there, sorting
-// candidates about 500 once; 100 000 x 300 with 5: 99 us against 125).  Longer ones are streamed: by
+// Rows of up to 2 KiB sit in the registers of 16 or 64 lanes (1 KiB from four alternatives on in
+// fp32, 512 bytes from nine on: finding them one by one costs 30 to 110 instructions each there,
+// sorting candidates about 500 once; 100 000 x 300 fp32 with 5: 99 us against 125, 41 943 x 800 fp16
+// with 5: 46 against 55, 83 886 x 400 fp16 with 32: 173 against 139).  Longer ones are streamed: by
 // a wavefront each where there are enough rows to fill the machine that way (256 CUs, 16
 // wavefronts each) and a row is not so long that its last wavefronts run alone; by a workgroup
 // each otherwise, split further until about four workgroups a CU run, none with less than 4096
 // entries (one tile of 16-bit loads is 8192, and a second launch joins the parts).
 LpPlan plan_forward(int rows, int vocab, int bytes, int top) {
-    if ((int64_t)vocab * bytes <= (top < 4 ? kShortBytes : top <= 8 ? kShortBytes / 2 : kShortBytes / 4)) return {0, 1, 0};
+    const int whole = bytes == 2 ? 8 : 3;   // alternatives for which a row may have all of kShortBytes
+    if ((int64_t)vocab * bytes <= (top <= whole ? kShortBytes : top <= 8 ? kShortBytes / 2 : kShortBytes / 4)) return {0, 1, 0};
     if (rows >= 4096 && vocab <= 8192) return {1, 1, 0};
     const int want = rows >= 512 ? 1 : (1024 + rows - 1) / rows;
     const int most = (vocab + 4095) / 4096;
