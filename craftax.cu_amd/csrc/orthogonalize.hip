@@ -18,11 +18,13 @@
 //   P = 3  every matrix is a pair hi + lo of fp16 numbers (22 bits, or to 2^-35 of 1) and a
 //          product is hi hi + hi lo + lo hi: what is left out, lo lo, is below 2^-22 of a
 //          product.  Error against 64 bits about 1e-6 of the result's norm, as fp32 has.
-//          For fp32 and fp16 inputs.
+//          What every input type gets unless the caller asks for less.
 //   P = 1  one fp16 product; X alone keeps its lo part, for the term a X.  Without it the
 //          rounding of X at every step is amplified by a (3.44) a step where singular values
-//          are small: 5e-3 of the norm measured instead of 1 to 2e-3, which is a bf16 rounding
-//          (1.7e-3).  A third of the matrix instructions.  For bf16 inputs.
+//          are small: 5e-3 of the norm measured instead of 1 to 2e-3.  A third of the matrix
+//          instructions (4096 x 4096 bf16: 1.46 ms, 3.56 with three), and only where the caller
+//          says so: what it loses, 7e-4 of the norm before the result is rounded, is not lost
+//          in a bf16 rounding (1.66e-3; together 1.80e-3).
 #include <utility>
 
 #include "cfp_internal.h"
@@ -1471,7 +1473,7 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
     CFP_REQUIRE((d_g == d_out && (ld == ld_out || rows == 1) && (batch_stride == out_batch_stride || batch == 1)) ||
                     apart(d_g, ld, batch_stride, d_out, ld_out, out_batch_stride, batch, rows, cols, type_bytes(dtype)),
                 "cfp_orthogonalize: the output may replace the input, with the same strides, but not overlap it otherwise");
-    const int p = products ? products : dtype == CFP_BF16 ? 1 : 3;
+    const int p = products ? products : 3;
     const Plan plan = make_plan(batch, rows, cols, p);
     CFP_REQUIRE(plan.total == 0 || (d_work && work_bytes >= plan.total && (reinterpret_cast<uintptr_t>(d_work) & 255u) == 0),
                 "cfp_orthogonalize: needs a 256-byte aligned workspace of %zu bytes (got %zu)", plan.total, work_bytes);

@@ -657,7 +657,8 @@ def _coefs_of(coefs, steps):
 
 def orthogonalize(g, steps=5, coefs=None, eps=1e-7, products=0, out=None):
     """Newton-Schulz products towards the nearest semi-orthogonal matrix of each matrix of g
-    (cfp_orthogonalize).  coefs: (a, b, c) or one triple a step."""
+    (cfp_orthogonalize).  coefs: (a, b, c) or one triple a step.  products: 0 or 3 for the accuracy
+    of fp32 whatever g's type, 1 for single fp16 products."""
     ptr, dtype, ld, stride, batch, rows, cols = _matrices_of(g, "g")
     dev = g.device
     if out is None:
@@ -665,7 +666,7 @@ def orthogonalize(g, steps=5, coefs=None, eps=1e-7, products=0, out=None):
     _need(out.shape == g.shape and out.dtype == g.dtype and out.device == dev,
           "out: g's shape, type and device expected")
     op, _, ldo, so, _, _, _ = _matrices_of(out, "out")
-    products = products or (1 if g.dtype == torch.bfloat16 else 3)
+    products = products or 3
     c = _coefs_of(coefs, steps)
     need = lib().cfp_orthogonalize_workspace(batch, rows, cols, products)
     work = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -453,9 +453,9 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
  * strides ld / ld_out and matrix strides batch_stride / out_batch_stride in elements (any for a
  * batch of one); d_out may be d_g with the same strides, any other overlap is an error.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315) for
  * every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
- * products: 1 = one fp16 matrix product per product (2e-3 of the result's norm from the 64-bit
- * result), 3 = three (1e-6, as fp32), 0 = by type: 1 for bf16, 3 for fp32 and fp16.  Sums are
- * fp32, the norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes all
+ * products: 3 (or 0) = three fp16 matrix products per product (1e-6 of the result's norm from the
+ * 64-bit result, as fp32 has), 1 = one (up to 2e-3, in a third of the time).  Sums are fp32, the
+ * norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes all
  * of it NaN.
  * d_work: cfp_orthogonalize_workspace(batch, rows, cols, products) bytes (products 1 or 3),
  * 256-byte aligned (may be NULL where that is 0: matrices that fit into one workgroup); calls that

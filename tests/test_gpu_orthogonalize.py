@@ -322,3 +322,18 @@ def test_refusals_with_device_tensors(pkg, cuda):
     with pytest.raises(pkg._lib.CfpError, match="overlap"):
         pol.orthogonalize(g[None].expand(3, 8, 12))
     assert pol.orthogonalize(torch.zeros(0, 4, 4, device=cuda)).numel() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 31, 33), (1, 128, 128), (9, 256, 256), (1, 256, 843), (2, 192, 700),
+                                             (1, 2050, 700), (1, 1024, 1024), (1, 64, 9000)])
+def test_fewer_bits_only_when_asked_for(pkg, cuda, dtype, batch, rows, cols):
+    """By default every type gets the accuracy of fp32 and one rounding to its own at the end.  With
+    e the error before that rounding, nearest(w + e) is at most |nearest(w) - w| + 2 |e| from w."""
+    torch = _torch()
+    g = gradient(cuda, batch, rows, cols, dtype, seed=3 * rows + cols)
+    want = reference(g)
+    once = off(want.to(g.dtype), want)
+    got = pkg.policy.orthogonalize(g)
+    assert off(got, want) <= once + 2 * (5e-6 + 2.0 ** -21 * np.sqrt(max(rows, cols))), (off(got, want), once)
+    assert torch.equal(got, pkg.policy.orthogonalize(g, products=3))
