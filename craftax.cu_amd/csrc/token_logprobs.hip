@@ -870,60 +870,65 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
 
 // Entries [lo, hi) of a row by one workgroup: what all entries have in common first, then the
 // named entries (given token, alternatives) once more by one lane each.  Their logits are read
-// before the first store, their values stored behind the last one (barriers on both sides), so
-// that dx may be x.
-template <typename T, bool MASK>
-__global__ __launch_bounds__(256) void k_logprobs_grad(LpGradArgs a) {
-    constexpr int N = Vec<T>::N, STRIDE = 256 * N, TILE = STRIDE * kU;
-    const int row = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
-    const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
-    const T* x = (const T*)a.x + (size_t)row * a.ld;
-    const uint8_t* mask = MASK ? a.mask + (size_t)row * a.ld_mask : nullptr;
-    T* dx = (T*)a.dx + (size_t)row * a.ld_dx;
-    const int lane = threadIdx.x & 63;
-    // every wavefront holds all named entries, one a lane (top <= 32)
-    float g;
-    const int named = named_entry<T>(a, row, lane, g);
-    RowGrad rg;
-    row_grad(a, row, sum_lanes<64>(g), rg);
-    float patch = 0.0f;
-    const bool mine = threadIdx.x < 64 && named >= lo && named < hi && !rg.none;
-    if (threadIdx.x < 64) {
-        patch = mine ? rg.at(to_f32(x[named])) : 0.0f;
-        for (int j = 0; j <= a.top; j++)   // an index that is named twice gets both gradients
-            if (__builtin_amdgcn_readlane(named, j) == named)
-                patch += lane_value(g, j);
-    }
-    __syncthreads();
-    int base = lo;
-    for (; base + TILE <= hi; base += TILE) {
-        const int i0 = base + (int)threadIdx.x * N;
-        Vec<T> raw[kU];
-        uint8_t mk[kU][N];
-#pragma unroll
-        for (int q = 0; q < kU; q++) {
-            raw[q] = load_vec(x + i0 + q * STRIDE);
-            if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
+// before the first store, their values stored behind the last one (barriers on both sides).  The
+// barriers order one workgroup only, and every workgroup of a row reads all of its named logits:
+// where dx is x, a row has one workgroup (plan_grad), of kInPlaceThreads.
+constexpr int kInPlaceThreads = 1024;
+template <typename T, bool MASK, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_logprobs_grad(LpGradArgs a) {
+    constexpr int N = Vec<T>::N, STRIDE = THREADS * N, TILE = STRIDE * kU;
+    const int64_t items = (int64_t)a.rows * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int row = (int)(item / a.splits), split = (int)(item % a.splits);
+        const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
+        const T* x = (const T*)a.x + (size_t)row * a.ld;
+        const uint8_t* mask = MASK ? a.mask + (size_t)row * a.ld_mask : nullptr;
+        T* dx = (T*)a.dx + (size_t)row * a.ld_dx;
+        const int lane = threadIdx.x & 63;
+        // every wavefront holds all named entries, one a lane (top <= 32)
+        float g;
+        const int named = named_entry<T>(a, row, lane, g);
+        RowGrad rg;
+        row_grad(a, row, sum_lanes<64>(g), rg);
+        float patch = 0.0f;
+        const bool mine = threadIdx.x < 64 && named >= lo && named < hi && !rg.none;
+        if (threadIdx.x < 64) {
+            patch = mine ? rg.at(to_f32(x[named])) : 0.0f;
+            for (int j = 0; j <= a.top; j++)   // an index that is named twice gets both gradients
+                if (__builtin_amdgcn_readlane(named, j) == named)
+                    patch += lane_value(g, j);
         }
+        __syncthreads();
+        int base = lo;
+        for (; base + TILE <= hi; base += TILE) {
+            const int i0 = base + (int)threadIdx.x * N;
+            Vec<T> raw[kU];
+            uint8_t mk[kU][N];
 #pragma unroll
-        for (int q = 0; q < kU; q++) {
-            Vec<T> out;
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const float xv = to_f32(raw[q].v[j]);
-                const bool on = !rg.none && !(MASK && mk[q][j] == 0) && !(xv == -INFINITY);
-                out.v[j] = (T)(on ? rg.at(xv) : 0.0f);
+            for (int q = 0; q < kU; q++) {
+                raw[q] = load_vec(x + i0 + q * STRIDE);
+                if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
             }
-            store_vec(dx + i0 + q * STRIDE, out);
+#pragma unroll
+            for (int q = 0; q < kU; q++) {
+                Vec<T> out;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const float xv = to_f32(raw[q].v[j]);
+                    const bool on = !rg.none && !(MASK && mk[q][j] == 0) && !(xv == -INFINITY);
+                    out.v[j] = (T)(on ? rg.at(xv) : 0.0f);
+                }
+                store_vec(dx + i0 + q * STRIDE, out);
+            }
         }
+        for (int i = base + (int)threadIdx.x; i < hi; i += THREADS) {
+            const float xv = to_f32(x[i]);
+            const bool on = !rg.none && !(MASK && mask[i] == 0) && !(xv == -INFINITY);
+            dx[i] = (T)(on ? rg.at(xv) : 0.0f);
+        }
+        __syncthreads();
+        if (mine) dx[named] = (T)patch;
     }
-    for (int i = base + (int)threadIdx.x; i < hi; i += 256) {
-        const float xv = to_f32(x[i]);
-        const bool on = !rg.none && !(MASK && mask[i] == 0) && !(xv == -INFINITY);
-        dx[i] = (T)(on ? rg.at(xv) : 0.0f);
-    }
-    __syncthreads();
-    if (mine) dx[named] = (T)patch;
 }
 
 // ---- plans --------------------------------------------------------------------------------
@@ -950,9 +955,11 @@ LpPlan plan_forward(int rows, int vocab, int bytes, int top) {
     splits = (vocab + chunk - 1) / chunk;
     return {2, splits, chunk};
 }
-// the gradient's parts are independent: 16384 entries a workgroup at most, 2048 at least
-LpPlan plan_grad(int rows, int vocab, int bytes) {
+// the gradient's parts are independent unless it replaces the logits: 16384 entries a workgroup at
+// most, 1024 at least
+LpPlan plan_grad(int rows, int vocab, int bytes, bool in_place) {
     if ((int64_t)vocab * bytes <= kShortBytes) return {0, 1, 0};
+    if (in_place) return {2, 1, vocab};
     int splits = (vocab + 16383) / 16384;
     while ((int64_t)rows * splits < 2048 && (vocab + splits - 1) / splits > 2048) splits *= 2;
     const int chunk = ((vocab + splits - 1) / splits + 7) / 8 * 8;
@@ -965,7 +972,10 @@ size_t part_bytes(int rows, int splits, int top) {
 constexpr int kMaxVocab = 1 << 30;
 // workgroups of a launch: threads of a grid are counted in 32 bits
 constexpr int64_t kMaxGroups = ((int64_t)1 << 32) / 256 - 1;
-int capped_groups(int64_t g) { return (int)(g < kMaxGroups ? g : kMaxGroups); }
+int capped_groups(int64_t g, int threads = 256) {
+    const int64_t most = kMaxGroups / (threads / 256);
+    return (int)(g < most ? g : most);
+}
 
 // one thread a row has no use for alternatives: 16 lanes find them together
 // (8: a vector of 16-bit logits)
@@ -1019,8 +1029,12 @@ void run_grad(const LpGradArgs& a, const LpPlan& pl, hipStream_t st) {
             else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
         }
     } else {
-        hipLaunchKernelGGL((k_logprobs_grad<T, MASK>), dim3((unsigned)((int64_t)a.rows * a.splits)), dim3(256), 0,
-                           st, a);
+        const int64_t items = (int64_t)a.rows * a.splits;
+        if (a.x == a.dx)
+            hipLaunchKernelGGL((k_logprobs_grad<T, MASK, kInPlaceThreads>), dim3(capped_groups(items, kInPlaceThreads)),
+                               dim3(kInPlaceThreads), 0, st, a);
+        else
+            hipLaunchKernelGGL((k_logprobs_grad<T, MASK, 256>), dim3(capped_groups(items)), dim3(256), 0, st, a);
     }
 }
 
@@ -1103,7 +1117,7 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
     const char* y1 = y0 + ((size_t)(rows - 1) * ld_dlogits + vocab) * elem_bytes(dtype);
     CFP_REQUIRE(y0 >= x1 || x0 >= y1 || (x0 == y0 && (ld == ld_dlogits || rows == 1)),
                 "cfp_token_logprobs_grad: the gradient may replace the logits, with the same stride, but not overlap them otherwise");
-    const LpPlan pl = plan_grad(rows, vocab, (int)elem_bytes(dtype));
+    const LpPlan pl = plan_grad(rows, vocab, (int)elem_bytes(dtype), d_logits == d_dlogits);
     CFP_REQUIRE(pl.kind < 2 || (int64_t)rows * pl.splits <= kMaxGroups, "cfp_token_logprobs_grad: %d rows of %d are more than one launch holds",
                 rows, vocab);
     LpGradArgs a{};

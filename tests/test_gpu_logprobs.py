@@ -445,3 +445,37 @@ def test_refusals_with_device_tensors(pkg, cuda):
         wide = torch.zeros(4, 90, device=cuda)
         pol.token_logprobs_backward(wide[:, :43], tok, st, out=wide[:, 20:63])
     assert pol.token_logprobs(x[:0], tok[:0]).logprobs.numel() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(1, 131072), (2, 50021), (7, 2100), (300, 40001), (3000, 17000)])
+def test_in_place_with_named_entries_that_are_not_allowed(pkg, cuda, dtype, rows, vocab):
+    """Tokens and alternatives at -inf, spread over the whole row, with gradients of their own: they
+    pass nothing on, whichever part of the row is replaced first.  In 16 bits some gradients that
+    replace a logit overflow to -inf.  Bit for bit as into another array."""
+    torch = _torch()
+    pol = pkg.policy
+    x, tok = make(cuda, dtype, rows, vocab, seed=21)
+    at = torch.arange(rows, device=cuda)
+    tok[:] = ((at * 7919 + vocab // 3) % vocab).int()
+    named = torch.stack([(at * 131 + k * (vocab // 9) + 5) % vocab for k in range(9)], 1).int()
+    off_ = at % 4 != 3                        # three rows of four: the token is not allowed
+    x[at[off_], tok[off_].long()] = -torch.inf
+    x.scatter_(1, named[:, ::2].long(), -torch.inf)
+    mask = None if dtype == "f32" else torch.ones(vocab, dtype=torch.uint8, device=cuda)
+    got = pol.token_logprobs(x, tok, mask=mask, stats=True)
+    g = torch.Generator(device="cpu").manual_seed(5)
+    g_lp, g_ent = (torch.randn(rows, generator=g).to(cuda) for _ in range(2))
+    g_lp *= 1e9 if dtype == "f16" else 1.0
+    g_top = torch.randn(rows, 9, generator=g).to(cuda)
+    for ids, gt in ((None, None), (named.contiguous(), g_top)):
+        kw = dict(g_logprobs=g_lp, g_entropy=g_ent, mask=mask, top_ids=ids, g_top=gt)
+        want = pol.token_logprobs_backward(x, tok, got.stats, **kw)
+        ref, tol = grad_reference(x[:8], tok[:8], mask, g_lp[:8], g_ent[:8], None if ids is None else ids[:8],
+                                  None if gt is None else gt[:8])
+        if dtype == "f32":
+            close(want[:8], ref, tol.numpy() + U * ref.abs().numpy() + 2.0 ** -149, "gradient")
+        for _ in range(3):
+            y = x.clone()
+            pol.token_logprobs_backward(y, tok, got.stats, out=y, **kw)
+            assert torch.equal(y, want)
