@@ -872,8 +872,11 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
 // named entries (given token, alternatives) once more by one lane each.  Their logits are read
 // before the first store, their values stored behind the last one (barriers on both sides).  The
 // barriers order one workgroup only, and every workgroup of a row reads all of its named logits:
-// where dx is x, a row has one workgroup (plan_grad), of kInPlaceThreads.
-constexpr int kInPlaceThreads = 1024;
+// where dx is x, a row has one workgroup (plan_grad), of kInPlaceThreads (bf16, in parts to another
+// array / in place by 256 / 512 / 1024 threads: 1 x 131 072 4 / 28 / 17 / 15 us, 128 x 131 072
+// 16 / 33 / 22 / 19, 2048 x 131 072 193 / 217 / 207 / 201, 4096 x 50 021 219 / 177 / 170 / 294,
+// 4096 x 4000 39 / 27 / 32 / 53).
+constexpr int kInPlaceThreads = 512;
 template <typename T, bool MASK, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_logprobs_grad(LpGradArgs a) {
     constexpr int N = Vec<T>::N, STRIDE = THREADS * N, TILE = STRIDE * kU;
