@@ -840,9 +840,9 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
         }
         __syncthreads();
         const int here = min(kRowsThreads, a.rows - r0) * pitch;
-        if (a.ld_dx == pitch && here % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
-            // rows without gaps, in LDS and in memory: one run of aligned vectors (r0 * pitch is a
-            // multiple of kRowsThreads)
+        if (a.ld_dx == a.vocab && pitch == a.vocab && here % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
+            // rows without gaps, in memory and (odd widths) in LDS: one run of aligned vectors (r0 * pitch
+            // is a multiple of kRowsThreads)
             T* dx = (T*)a.dx + (size_t)r0 * pitch;
 #pragma unroll 4
             for (int e = (int)threadIdx.x * N; e < here; e += kRowsThreads * N) {

@@ -479,3 +479,24 @@ def test_in_place_with_named_entries_that_are_not_allowed(pkg, cuda, dtype, rows
             y = x.clone()
             pol.token_logprobs_backward(y, tok, got.stats, out=y, **kw)
             assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(16384, 8), (16384, 42), (16500, 42), (16512, 64), (16391, 10)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_one_column_behind_even_rows_is_left_alone(pkg, cuda, dtype, rows, vocab, in_place):
+    """Rows vocab + 1 apart, as a head's logits with a value behind them: the gradient leaves that
+    column and what follows the last logit as they were."""
+    torch = _torch()
+    x, tok = make(cuda, dtype, rows, vocab, ld=vocab + 1, seed=vocab)
+    got = pkg.policy.token_logprobs(x, tok, stats=True)
+    g = torch.randn(rows, generator=torch.Generator().manual_seed(2)).to(cuda)
+    want = pkg.policy.token_logprobs_backward(x.contiguous(), tok, got.stats, g_logprobs=g, g_entropy=g)
+    store = torch.full((rows * (vocab + 1) + 64,), 9.0, dtype=x.dtype, device=cuda)
+    out = store[:rows * (vocab + 1)].view(rows, vocab + 1)[:, :vocab]
+    assert out.data_ptr() % 16 == 0
+    if in_place:
+        out.copy_(x)
+    dx = pkg.policy.token_logprobs_backward(out if in_place else x, tok, got.stats, g_logprobs=g, g_entropy=g, out=out)
+    assert torch.equal(dx, want)
+    assert store[:rows * (vocab + 1)].view(rows, vocab + 1)[:, vocab].eq(9).all() and store[rows * (vocab + 1) - 1:].eq(9).all()
