@@ -354,10 +354,9 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
     constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
-    for (int row0 = (int)blockIdx.x * per; row0 < a.rows; row0 += (int)gridDim.x * per) {
-        const int row = row0 + (int)threadIdx.x / L;
-        const bool live = row < a.rows;
-        const int r = live ? row : a.rows - 1;
+    for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
+        const bool live = row0 + (int)threadIdx.x / L < a.rows;
+        const int r = live ? (int)row0 + (int)threadIdx.x / L : a.rows - 1;
         const int tok = a.tok[r];
         const float xt = token_logit<T>(a, r, tok);
         float v[Q][N];
@@ -376,7 +375,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
             for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
         z.s = sum_lanes<L>(z.s);
         z.u = sum_lanes<L>(z.u);
-        if (live && sub == 0) write_row(a, row, z, tok, xt);
+        if (live && sub == 0) write_row(a, r, z, tok, xt);
         if (a.top == 0) continue;
         // Alternatives: the maximum of the row, then the lowest index that holds it, `top` times; lane
         // k (then k - L) keeps number k, and all are written together.  16-bit entries and their index
@@ -413,7 +412,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
 #pragma unroll
             for (int t = 0; t < SLOTS; t++)
                 if (live && t * L + sub < a.top)
-                    write_top(a, row, z, t * L + sub, kept[t] ? key_of(short_value<T>(kept[t]), 0xffff - (int)(kept[t] & 0xffffu)) : 0);
+                    write_top(a, r, z, t * L + sub, kept[t] ? key_of(short_value<T>(kept[t]), 0xffff - (int)(kept[t] & 0xffffu)) : 0);
             continue;
         }
         uint64_t kept[SLOTS] = {};
@@ -438,7 +437,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
         }
 #pragma unroll
         for (int t = 0; t < SLOTS; t++)
-            if (live && t * L + sub < a.top) write_top(a, row, z, t * L + sub, kept[t]);
+            if (live && t * L + sub < a.top) write_top(a, r, z, t * L + sub, kept[t]);
     }
 }
 
@@ -467,7 +466,7 @@ struct RowVectors {
 // Rows [r0, r0 + kRowsThreads) of x as fp32 into LDS, -inf where masked; all of a thread's loads in
 // flight together (at most PASSES; per_row of them).
 template <typename T, int PASSES, bool MASK>
-__device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t* mask, int64_t ld_mask, int r0, int rows,
+__device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t* mask, int64_t ld_mask, int64_t r0, int rows,
                                            int vocab, float* stage) {
     constexpr int N = Vec<T>::N;
     const RowVectors<N> rv(vocab);
@@ -494,8 +493,8 @@ __device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t
 template <typename T, int PASSES, bool MASK>
 __global__ __launch_bounds__(kRowsThreads) void k_logprobs_rows(LpArgs a) {
     extern __shared__ float stage[];
-    for (int r0 = (int)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int)gridDim.x * kRowsThreads) {
-        const int row = r0 + (int)threadIdx.x;
+    for (int64_t r0 = (int64_t)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int64_t)gridDim.x * kRowsThreads) {
+        const int64_t row = r0 + (int)threadIdx.x;
         stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
         const int tok = row < a.rows ? a.tok[row] : -1;
         __syncthreads();
@@ -506,7 +505,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_rows(LpArgs a) {
             for (int i = 0; i < a.vocab; i++) z.m = fmaxf(z.m, x[i]);
 #pragma unroll 4
             for (int i = 0; i < a.vocab; i++) add_entry(z, x[i]);
-            write_row(a, row, z, tok, tok >= 0 && tok < a.vocab ? x[tok] : -INFINITY);
+            write_row(a, (int)row, z, tok, tok >= 0 && tok < a.vocab ? x[tok] : -INFINITY);
         }
         __syncthreads();
     }
@@ -621,9 +620,9 @@ template <typename T, bool MASK, bool TOP>
 __global__ __launch_bounds__(256) void k_logprobs_wave(LpArgs a) {
     __shared__ TopSpace spaces[TOP ? 4 : 1];
     const int lane = threadIdx.x & 63;
-    for (int row0 = (int)blockIdx.x * 4; row0 < a.rows; row0 += (int)gridDim.x * 4) {
-        const int row = row0 + (int)(threadIdx.x >> 6);
-        if (row >= a.rows) return;   // whole wavefronts; nothing below synchronises a workgroup
+    for (int64_t row0 = (int64_t)blockIdx.x * 4; row0 < a.rows; row0 += (int64_t)gridDim.x * 4) {
+        if (row0 + (threadIdx.x >> 6) >= a.rows) return;   // whole wavefronts; nothing below synchronises a workgroup
+        const int row = (int)row0 + (int)(threadIdx.x >> 6);
         const int tok = a.tok[row];
         const float xt = token_logit<T>(a, row, tok);
         Sums z;
@@ -765,10 +764,9 @@ __global__ __launch_bounds__(256) void k_logprobs_grad_short(LpGradArgs a) {
     constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
     const int per = 256 / L;
-    for (int row0 = (int)blockIdx.x * per; row0 < a.rows; row0 += (int)gridDim.x * per) {
-        const int row = row0 + (int)threadIdx.x / L;
-        const bool live = row < a.rows;
-        const int r = live ? row : a.rows - 1;
+    for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
+        const bool live = row0 + (int)threadIdx.x / L < a.rows;
+        const int r = live ? (int)row0 + (int)threadIdx.x / L : a.rows - 1;
         float v[Q][N], d[Q][N];
         int first[Q];
         load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
@@ -820,8 +818,8 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
     extern __shared__ float stage[];
     constexpr int N = Vec<T>::N;
     const int pitch = rows_pitch(a.vocab);
-    for (int r0 = (int)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int)gridDim.x * kRowsThreads) {
-        const int row = r0 + (int)threadIdx.x;
+    for (int64_t r0 = (int64_t)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int64_t)gridDim.x * kRowsThreads) {
+        const int64_t row = r0 + (int)threadIdx.x;
         stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
         int tok = -1;
         float g = 0.0f;
@@ -831,7 +829,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
             float* x = stage + threadIdx.x * pitch;
             const bool hit = tok >= 0 && tok < a.vocab && !(x[tok] == -INFINITY);
             RowGrad rg;
-            row_grad(a, row, tok >= a.vocab ? NAN : hit ? g : 0.0f, rg);
+            row_grad(a, (int)row, tok >= a.vocab ? NAN : hit ? g : 0.0f, rg);
 #pragma unroll 4
             for (int i = 0; i < a.vocab; i++) {
                 const float v = x[i];
@@ -839,7 +837,7 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
             }
         }
         __syncthreads();
-        const int here = min(kRowsThreads, a.rows - r0) * pitch;
+        const int here = (int)min((int64_t)kRowsThreads, a.rows - r0) * pitch;
         if (a.ld_dx == a.vocab && pitch == a.vocab && here % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
             // rows without gaps, in memory and (odd widths) in LDS: one run of aligned vectors (r0 * pitch
             // is a multiple of kRowsThreads)
@@ -973,7 +971,8 @@ size_t part_bytes(int rows, int splits, int top) {
 }
 
 constexpr int kMaxVocab = 1 << 30;
-// workgroups of a launch: threads of a grid are counted in 32 bits
+// workgroups of a launch: threads of a grid are counted in 32 bits.  (Rows are counted in 64 bits by
+// the loops over them: the last workgroup's next row is up to twice their number.)
 constexpr int64_t kMaxGroups = ((int64_t)1 << 32) / 256 - 1;
 int capped_groups(int64_t g, int threads = 256) {
     const int64_t most = kMaxGroups / (threads / 256);

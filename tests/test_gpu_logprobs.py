@@ -500,3 +500,36 @@ def test_one_column_behind_even_rows_is_left_alone(pkg, cuda, dtype, rows, vocab
     dx = pkg.policy.token_logprobs_backward(out if in_place else x, tok, got.stats, g_logprobs=g, g_entropy=g, out=out)
     assert torch.equal(dx, want)
     assert store[:rows * (vocab + 1)].view(rows, vocab + 1)[:, vocab].eq(9).all() and store[rows * (vocab + 1) - 1:].eq(9).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [((1 << 30) + 300, 8), ((1 << 31) - 1, 2)])
+def test_row_counts_past_30_bits(pkg, cuda, rows, vocab):
+    """More rows than a 32-bit loop over them can step past, by one thread a row and by lanes: rows at
+    the start, around 2^30 and at the end as in a call of their own, bit for bit."""
+    torch = _torch()
+    pol = pkg.policy
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GiB of free GPU memory")
+    part = 16384 + 77
+    cuts = [slice(a, a + part) for a in (0, (1 << 30) - part // 2, rows - part)]
+    cuts = [c for c in cuts if c.stop <= rows]
+    x = torch.zeros((rows, vocab), dtype=torch.float16, device=cuda)
+    tok = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    g = torch.zeros(rows, dtype=torch.float32, device=cuda)
+    for c in cuts:
+        x[c] = torch.randn(part, vocab, device=cuda).half()
+        tok[c] = torch.randint(-1, vocab, (part,), dtype=torch.int32, device=cuda)
+        g[c] = torch.randn(part, device=cuda)
+    got = pol.token_logprobs(x, tok, stats=True)
+    dx = pol.token_logprobs_backward(x, tok, got.stats, g_logprobs=g, g_entropy=g)
+    for c in cuts:
+        want = pol.token_logprobs(x[c].clone(), tok[c].clone(), stats=True)
+        for a, b in ((got.logprobs, want.logprobs), (got.entropy, want.entropy), (got.stats, want.stats)):
+            assert torch.equal(a[c], b)
+        assert torch.equal(dx[c], pol.token_logprobs_backward(x[c].clone(), tok[c].clone(), want.stats, g_logprobs=g[c].clone(),
+                                                              g_entropy=g[c].clone()))
+    middle = slice(rows // 4, rows // 4 + 1000)      # equal logits, token 0
+    assert (got.logprobs[middle] + np.log(vocab)).abs().max().item() <= 8 * U
+    del x, tok, g, got, dx
+    torch.cuda.empty_cache()
