@@ -1120,8 +1120,6 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
     CFP_REQUIRE(y0 >= x1 || x0 >= y1 || (x0 == y0 && (ld == ld_dlogits || rows == 1)),
                 "cfp_token_logprobs_grad: the gradient may replace the logits, with the same stride, but not overlap them otherwise");
     const LpPlan pl = plan_grad(rows, vocab, (int)elem_bytes(dtype), d_logits == d_dlogits);
-    CFP_REQUIRE(pl.kind < 2 || (int64_t)rows * pl.splits <= kMaxGroups, "cfp_token_logprobs_grad: %d rows of %d are more than one launch holds",
-                rows, vocab);
     LpGradArgs a{};
     a.x = d_logits; a.ld = ld; a.rows = rows; a.vocab = vocab; a.tok = d_tokens;
     a.mask = d_mask; a.ld_mask = ld_mask; a.stats = d_stats;

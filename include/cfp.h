@@ -420,7 +420,8 @@ enum cfp_dtype { CFP_F32 = 0, CFP_BF16 = 1, CFP_F16 = 2 };
  *   d_stats[r][3]     what cfp_token_logprobs_grad needs (NULL = not written)
  * A row that allows nothing has log-probability -inf, entropy 0 and no alternatives; a row with
  * NaN or +inf among its allowed logits has NaN and ids -1.  rows = 0 does nothing.
- * Logits need the alignment of their type only.  ld >= vocab (any ld for one row).
+ * Logits need the alignment of their type only.  ld >= vocab (any ld for one row).  2^24 - 1 rows of
+ * more than 8192 entries at most; shorter ones, and the gradient, any number.
  * d_work: cfp_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte aligned (may be NULL
  * where that is 0); calls that may overlap need one each. */
 size_t cfp_token_logprobs_workspace(int rows, int vocab, int top);

@@ -533,3 +533,35 @@ def test_row_counts_past_30_bits(pkg, cuda, rows, vocab):
     assert (got.logprobs[middle] + np.log(vocab)).abs().max().item() <= 8 * U
     del x, tok, g, got, dx
     torch.cuda.empty_cache()
+
+
+def test_what_can_be_scored_can_be_differentiated(pkg, cuda):
+    """More rows too long for registers than one launch has workgroups."""
+    torch = _torch()
+    pol = pkg.policy
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GiB of free GPU memory")
+    rows, vocab, part = (1 << 24) + 4000, 1025, 5000
+    cuts = [slice(0, part), slice(rows - part, rows)]
+    x = torch.zeros((rows, vocab), dtype=torch.bfloat16, device=cuda)
+    tok = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    g = torch.ones(rows, device=cuda)
+    for c in cuts:
+        x[c] = torch.randn(part, vocab, device=cuda).bfloat16()
+        tok[c] = torch.randint(-1, vocab, (part,), dtype=torch.int32, device=cuda)
+        g[c] = torch.randn(part, device=cuda)
+    keep = [x[c].clone() for c in cuts]
+    got = pol.token_logprobs(x, tok, stats=True)
+    dx = pol.token_logprobs_backward(x, tok, got.stats, g_logprobs=g, g_entropy=g)
+    pol.token_logprobs_backward(x, tok, got.stats, g_logprobs=g, g_entropy=g, out=x)
+    fi = torch.finfo(torch.bfloat16)
+    for c, k in zip(cuts, keep):
+        assert torch.equal(dx[c], x[c])
+        want, tol = grad_reference(k, tok[c], None, g[c], g[c], None, None)
+        close(dx[c], want, tol.numpy() * (1 + fi.eps) + want.abs().numpy() * fi.eps / 2 + fi.tiny * fi.eps / 2, "gradient")
+    middle = dx[rows // 2]                      # equal logits, token 0: 1 - 1/1025, rounded to 1
+    assert middle[0].item() == 1.0 and (middle[1:].float() + 1 / vocab).abs().max().item() <= 2.0 ** -8 / vocab
+    del x
+    del dx, got
+    torch.cuda.empty_cache()
