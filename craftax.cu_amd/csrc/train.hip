@@ -758,6 +758,7 @@ int cfp_train_zero_loss(cfp_trainer* tr, void* stream) {
 
 int cfp_train_adam(cfp_trainer* tr, void* stream) {
     CFP_REQUIRE(tr, "cfp_train_adam: NULL trainer");
+    CFP_REQUIRE(tr->optimizer == CFP_OPT_ADAM, "cfp_train_adam: the trainer's optimiser is Muon, whose momentum the first moment holds (cfp_train_set_optimizer)");
     hipStream_t st = (hipStream_t)stream;
     // parameters, moments and every weight mirror of the forward kernels in one pass
     if (launch_adam(tr->p, tr->grads, tr->adam_m, tr->adam_v, tr->adam_ctr, tr->d_lr, 0.9f, 0.999f,

@@ -599,7 +599,8 @@ int cfp_train_adv_stats(cfp_trainer* tr, void* stream);
 int cfp_train_backward(cfp_trainer* tr, int env_start, int env_count, void* stream);
 int cfp_train_zero_loss(cfp_trainer* tr, void* stream);
 /* cu_train_adam (craftax_full.cu:13337): Adam step from the grads arena (which
- * it zeroes), bumps the step counter, rebuilds the weight mirrors. */
+ * it zeroes), bumps the step counter, rebuilds the weight mirrors.  The trainer's optimiser must
+ * be CFP_OPT_ADAM. */
 int cfp_train_adam(cfp_trainer* tr, void* stream);
 /* The optimiser of cfp_train_update's steps: CFP_OPT_ADAM (the default, the reference's) or
  * CFP_OPT_MUON (no counterpart in the reference): the weight matrices -- W_enc and, of every

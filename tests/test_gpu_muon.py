@@ -217,3 +217,27 @@ def test_the_operators_as_a_training_step_uses_them(pkg, cuda):
         assert ((w0.double().cpu() - o) - w.double().cpu()).norm() <= tol * o.norm() + 3 * 2.0 ** -24 * w0.double().cpu().norm()
     assert got.top_ids.shape == (n, 3) and (got.top_logprobs[:, :1] >= got.logprobs[:, None] - 1e-5).all()
     pol.close()
+
+
+def test_an_adam_step_of_a_muon_trainer_is_refused(pkg, cuda):
+    """Its first moment holds Muon's momentum: nothing may change."""
+    import torch
+    pol = pkg.Policy(32, 1, seed=4)
+    tr = pkg.Trainer(pol, 2)
+    tr.set_optimizer("muon")
+    g = torch.randn(pol.param_count, device=cuda)
+    tr.buf("grads").copy_(g)
+    tr.muon()
+    tr.buf("grads").copy_(g)
+    before = pol.get_params(), tr.buf("adam_m").clone(), tr.buf("adam_v").clone()
+    with pytest.raises(pkg._lib.CfpError, match="optimiser is Muon"):
+        tr.adam()
+    torch.cuda.synchronize()
+    assert np.array_equal(pol.get_params(), before[0]) and torch.equal(tr.buf("grads"), g)
+    assert torch.equal(tr.buf("adam_m"), before[1]) and torch.equal(tr.buf("adam_v"), before[2])
+    tr.set_optimizer("adam")
+    tr.buf("grads").copy_(g)
+    tr.adam()
+    torch.cuda.synchronize()
+    assert not np.array_equal(pol.get_params(), before[0])
+    tr.close(); pol.close()
