@@ -1,6 +1,8 @@
 // Library-internal definition of the policy object (opaque in include/cfp.h).
 #pragma once
 
+#include <numeric>
+
 #include "cfp_common.h"
 
 struct cfp_policy {
@@ -45,6 +47,25 @@ int value_sample(const float* d_av, int n, int actions, float* d_env_actions, in
 // launch_forward also draws the actions (FwdArgs::s_act ...) when this holds: full-game
 // records in recording mode on 32-env tiles, one tile per workgroup (at most one per CU).
 bool forward_draws(const FwdArgs& a);
+
+// Whether two batches of `batch` matrices rows x cols (elements of `bytes`, row strides ld, matrix
+// strides `stride`) share no entry, where that shows: address ranges apart, or whole matrices or
+// columns side by side in a period that all strides are multiples of.
+inline bool apart(const void* a, int64_t ld_a, int64_t stride_a, const void* b, int64_t ld_b, int64_t stride_b, int batch, int rows,
+                  int cols, size_t bytes) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const int64_t span_a = (int64_t)(rows - 1) * ld_a + cols, span_b = (int64_t)(rows - 1) * ld_b + cols;
+    const uintptr_t a1 = a0 + ((batch - 1) * stride_a + span_a) * bytes, b1 = b0 + ((batch - 1) * stride_b + span_b) * bytes;
+    if (a1 <= b0 || b1 <= a0) return true;
+    const int64_t d = (int64_t)(b0 - a0) / (int64_t)bytes;
+    auto beside = [d](int64_t period, int64_t len_a, int64_t len_b) {
+        if (period <= 0) return false;
+        const int64_t from = (d % period + period) % period;
+        return from >= len_a && from <= period - len_b;
+    };
+    const int64_t matrices = batch > 1 ? std::gcd(stride_a, stride_b) : 0, lines = rows > 1 ? std::gcd(ld_a, ld_b) : 0;
+    return beside(matrices, span_a, span_b) || beside(std::gcd(matrices, lines), cols, cols);
+}
 
 // One Muon step of a batch of fp32 matrices that share ld and stride (orthogonalize.hip,
 // cfp_muon_update); clear_g: the gradient is zeroed behind its last read.

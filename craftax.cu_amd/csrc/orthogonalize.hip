@@ -1421,23 +1421,6 @@ void fill_coef(const float* coefs, int steps, float (&c)[3 * kMaxSteps]) {
     for (int i = 0; i < 3 * steps; i++) c[i] = coefs ? coefs[i] : kQuintic[i % 3];
 }
 size_t type_bytes(int dtype) { return dtype == CFP_F32 ? 4 : 2; }
-// Whether two batches of matrices share no entry: address ranges apart, or the same strides with
-// whole matrices or columns side by side.
-bool apart(const void* a, int64_t ld_a, int64_t stride_a, const void* b, int64_t ld_b, int64_t stride_b, int batch, int rows,
-           int cols, size_t bytes) {
-    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
-    const int64_t span_a = (int64_t)(rows - 1) * ld_a + cols, span_b = (int64_t)(rows - 1) * ld_b + cols;
-    const uintptr_t a1 = a0 + ((batch - 1) * stride_a + span_a) * bytes, b1 = b0 + ((batch - 1) * stride_b + span_b) * bytes;
-    if (a1 <= b0 || b1 <= a0) return true;
-    const int64_t d = (int64_t)((a0 > b0 ? a0 - b0 : b0 - a0) / bytes);
-    auto beside = [d](int64_t period, int64_t length) { return period > 0 && d % period >= length && d % period <= period - length; };
-    if (batch > 1) {
-        if (stride_a != stride_b) return false;
-        if (span_a == span_b && beside(stride_a, span_a)) return true;
-        if (ld_a < 1 || stride_a % ld_a) return false;
-    }
-    return ld_a == ld_b && beside(ld_a, cols);
-}
 
 }  // namespace
 }  // namespace cfp

@@ -1114,10 +1114,8 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
                 vocab, (long long)ld_dlogits);
     CFP_REQUIRE((reinterpret_cast<uintptr_t>(d_dlogits) & (dtype == CFP_F32 ? 3u : 1u)) == 0,
                 "cfp_token_logprobs_grad: output not aligned to its type");
-    const char *x0 = (const char*)d_logits, *y0 = (const char*)d_dlogits;
-    const char* x1 = x0 + ((size_t)(rows - 1) * ld + vocab) * elem_bytes(dtype);
-    const char* y1 = y0 + ((size_t)(rows - 1) * ld_dlogits + vocab) * elem_bytes(dtype);
-    CFP_REQUIRE(y0 >= x1 || x0 >= y1 || (x0 == y0 && (ld == ld_dlogits || rows == 1)),
+    CFP_REQUIRE((d_logits == d_dlogits && (ld == ld_dlogits || rows == 1)) ||
+                    apart(d_logits, ld, 0, d_dlogits, ld_dlogits, 0, 1, rows, vocab, elem_bytes(dtype)),
                 "cfp_token_logprobs_grad: the gradient may replace the logits, with the same stride, but not overlap them otherwise");
     const LpPlan pl = plan_grad(rows, vocab, (int)elem_bytes(dtype), d_logits == d_dlogits);
     LpGradArgs a{};

@@ -438,7 +438,7 @@ int cfp_token_logprobs(const void* d_logits, int dtype, int64_t ld, int rows, in
  * entry of a row that allows nothing.  A log-probability that is the constant 0 or -inf passes
  * no gradient on (negative or not allowed token, id -1); an index >= vocab makes the row's
  * allowed entries NaN.  d_dlogits may be d_logits itself with the same stride (the logits are
- * replaced); any other overlap is an error. */
+ * replaced) or columns beside them in the same rows; an overlap is an error. */
 int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int rows, int vocab,
                             const int32_t* d_tokens, const uint8_t* d_mask, int64_t ld_mask,
                             const float* d_stats, const float* d_g_logprobs, const float* d_g_entropy,

@@ -565,3 +565,27 @@ def test_what_can_be_scored_can_be_differentiated(pkg, cuda):
     del x
     del dx, got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(40, 43), (5, 2500), (2, 30001), (16400, 40)])
+def test_logits_and_gradient_as_columns_of_one_array(pkg, cuda, dtype, rows, vocab):
+    """Side by side in rows of one array, and in every second row of it: no entry is shared."""
+    torch = _torch()
+    pol = pkg.policy
+    x, tok = make(cuda, dtype, rows, vocab, seed=31)
+    got = pol.token_logprobs(x, tok, stats=True)
+    g = torch.randn(rows, generator=torch.Generator().manual_seed(4)).to(cuda)
+    want = pol.token_logprobs_backward(x, tok, got.stats, g_logprobs=g, g_entropy=g)
+    store = torch.full((rows, 4 * vocab), 9.0, dtype=x.dtype, device=cuda)
+    for a, b in ((store[:, :vocab], store[:, vocab:2 * vocab]), (store[:, 2 * vocab:3 * vocab], store[:, :vocab]),
+                 (store.view(2 * rows, 2 * vocab)[:rows, :vocab], store[:, vocab:2 * vocab])):
+        store.fill_(9.0)
+        a.copy_(x)
+        assert pol.token_logprobs_backward(a, tok, got.stats, g_logprobs=g, g_entropy=g, out=b) is b
+        assert torch.equal(b, want) and torch.equal(a, x)
+        a.fill_(9.0); b.fill_(9.0)
+        assert store.eq(9).all()
+    for b in (store[:, vocab - 1:2 * vocab - 1], store.view(2 * rows, 2 * vocab)[:rows, 1:vocab + 1]):
+        with pytest.raises(pkg._lib.CfpError, match="overlap"):
+            pol.token_logprobs_backward(store[:, :vocab], tok, got.stats, g_logprobs=g, out=b)
