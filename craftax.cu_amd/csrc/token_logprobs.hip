@@ -11,8 +11,9 @@
 // The forward reads the logits once (running maximum and sums, rescaled when the maximum
 // grows), the gradient reads them once and writes as many values: both are bound by HBM.
 // lp is taken from x_t - m and ln s, never from x_t - (m + ln s): with logits of 1e4 the sum
-// m + ln s has lost the bits of ln s.  All sums are fp32 per lane (at most a few hundred terms
-// each, in [0, 1]) and joined in a tree of fixed shape: the same call gives the same bits.
+// m + ln s has lost the bits of ln s.  All sums are fp32 per lane, of 512 terms in [0, 1] and the
+// entries of one more tile at most (rows above 2^17 entries are split for it), and joined in a tree of
+// fixed shape: the same call gives the same bits.
 #include <float.h>
 #include <limits.h>
 
@@ -944,14 +945,17 @@ struct LpPlan {
 // a wavefront each where there are enough rows to fill the machine that way (256 CUs, 16
 // wavefronts each) and a row is not so long that its last wavefronts run alone; by a workgroup
 // each otherwise, split further until about four workgroups a CU run, none with less than 4096
-// entries (one tile of 16-bit loads is 8192, and a second launch joins the parts).
+// entries (one tile of 16-bit loads is 8192, and a second launch joins the parts).  Parts hold at most
+// kMostEntries, 512 a lane: roundings of a longer running sum of equal terms all go one way (2.3e-4 of
+// the sum after 16 384 terms).
+constexpr int kMostEntries = 512 * 64 * kWaves;
 LpPlan plan_forward(int rows, int vocab, int bytes, int top) {
     const int whole = bytes == 2 ? 8 : 3;   // alternatives for which a row may have all of kShortBytes
     if ((int64_t)vocab * bytes <= (top <= whole ? kShortBytes : top <= 8 ? kShortBytes / 2 : kShortBytes / 4)) return {0, 1, 0};
     if (rows >= 4096 && vocab <= 8192) return {1, 1, 0};
     const int want = rows >= 512 ? 1 : (1024 + rows - 1) / rows;
-    const int most = (vocab + 4095) / 4096;
-    int splits = want < most ? want : most;
+    const int most = (vocab + 4095) / 4096, least = (vocab + kMostEntries - 1) / kMostEntries;
+    int splits = want < least ? least : want < most ? want : most;
     const int chunk = ((vocab + splits - 1) / splits + 7) / 8 * 8;
     splits = (vocab + chunk - 1) / chunk;
     return {2, splits, chunk};

@@ -589,3 +589,24 @@ def test_logits_and_gradient_as_columns_of_one_array(pkg, cuda, dtype, rows, voc
     for b in (store[:, vocab - 1:2 * vocab - 1], store.view(2 * rows, 2 * vocab)[:rows, 1:vocab + 1]):
         with pytest.raises(pkg._lib.CfpError, match="overlap"):
             pol.token_logprobs_backward(store[:, :vocab], tok, got.stats, g_logprobs=g, out=b)
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [("bf16", 513, 1 << 22), ("f16", 1, 1 << 30), ("f32", 700, 1000003)])
+def test_long_rows_keep_their_sums(pkg, cuda, dtype, rows, vocab):
+    """One entry at 0 and all others at -0.65625, whose exponentials round the same way at every step
+    of a long running sum (16 384 of them in a row: 2.3e-4).  A lane adds up 512 and part of a tile."""
+    torch = _torch()
+    torch.cuda.empty_cache()
+    x = torch.full((rows, vocab), -0.65625, dtype=getattr(torch, DT[dtype]), device=cuda)
+    tok = ((torch.arange(rows, device=cuda) * 7919) % vocab).int()
+    x[torch.arange(rows, device=cuda), tok.long()] = 0.0
+    got = pkg.policy.token_logprobs(x, tok, top=1)
+    rest = (vocab - 1) * np.exp(-0.65625)
+    ls = np.log1p(rest)
+    ent = ls + rest * 0.65625 / (1 + rest)
+    tol = U * (4 * 0.65625 + 2 * (512 + 64) + 32)
+    assert (got.logprobs.double() + ls).abs().max().item() <= tol + 4 * U * ls
+    assert (got.entropy.double() - ent).abs().max().item() <= tol * (1 + ent)
+    assert torch.equal(got.top_ids[:, 0], tok) and torch.equal(got.top_logprobs[:, 0], got.logprobs)
+    del x
+    torch.cuda.empty_cache()
