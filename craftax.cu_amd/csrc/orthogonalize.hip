@@ -1477,6 +1477,7 @@ namespace cfp {
 
 int muon_update(const MuonArgs& u, hipStream_t st) {
     if (check_sizes("cfp_muon_update", u.batch, u.rows, u.cols, u.steps, u.products, u.eps)) return 1;
+    CFP_REQUIRE(u.scale >= 0.0f, "cfp_muon_update: scale must not be negative (got %g)", (double)u.scale);
     if (u.batch == 0) return 0;
     CFP_REQUIRE(u.w && u.g && u.mom, "cfp_muon_update: NULL weight, gradient or momentum");
     CFP_REQUIRE(u.ld >= u.cols || (u.rows == 1 && u.ld >= 0), "cfp_muon_update: rows of %d need a stride of at least that (got %lld)",

@@ -99,3 +99,12 @@ def test_optimizer_refusals(pkg):
     assert lib.cfp_muon_defaults(None) != 0
     assert lib.cfp_train_set_optimizer(None, 1, None, None) != 0 and b"NULL" in lib.cfp_last_error()
     assert lib.cfp_train_muon(None, None) != 0 and lib.cfp_train_optimizer(None) == -1
+
+
+@pytest.mark.parametrize("scale", [-1.0, -1e-30, float("nan")])
+def test_muon_refuses_a_scale_below_zero(pkg, scale):
+    """0 asks for the default; below it nothing is meant."""
+    lib = pkg.lib()
+    far = [C.c_void_p(0x10000 + k * BIG) for k in range(3)]
+    assert lib.cfp_muon_update(*far, 64, 4096, 1, 64, 64, None, 0.1, 0.9, 1, 0.0, scale, 5, None, 1e-7, 0, P, BIG, None) != 0
+    assert b"scale" in lib.cfp_last_error()
