@@ -1505,6 +1505,7 @@ int muon_update(const MuonArgs& u, hipStream_t st) {
     out.out = u.w; out.dtype = CFP_F32; out.ld = u.ld; out.stride = u.stride;
     out.rows = u.rows; out.cols = u.cols; out.tall = u.rows > u.cols;
     out.update = 1; out.lr_dev = u.lr_dev; out.lr = u.lr; out.decay = u.decay;
+    // 0: sqrt(outputs / inputs) where that is above 1, of a weight [outputs][inputs]
     out.scale = u.scale > 0.0f ? u.scale : u.rows > u.cols ? sqrtf((float)u.rows / (float)u.cols) : 1.0f;
     return p == 3 ? run_all<3>(in, out, u.batch, u.steps, c, plan, (char*)u.work, st)
                   : run_all<1>(in, out, u.batch, u.steps, c, plan, (char*)u.work, st);

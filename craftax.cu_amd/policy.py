@@ -680,7 +680,8 @@ def orthogonalize(g, steps=5, coefs=None, eps=1e-7, products=0, out=None):
 def muon_update(w, g, momentum_buffer, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=0.0, steps=5,
                 coefs=None, eps=1e-7, products=0):
     """One Muon step on fp32 weights w in place (cfp_muon_update); momentum_buffer is updated too.
-    lr: a number, or a one-element fp32 tensor on the GPU (read when the step runs)."""
+    lr: a number, or a one-element fp32 tensor on the GPU (read when the step runs).  scale 0:
+    sqrt(max(1, rows / cols)), for weights [outputs][inputs]; [inputs][outputs] take theirs as a number."""
     ptr, dtype, ld, stride, batch, rows, cols = _matrices_of(w, "w")
     dev = w.device
     for t, name in ((g, "g"), (momentum_buffer, "momentum_buffer")):

@@ -471,7 +471,8 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
  *   m = momentum m + g,   u = g + momentum m (nesterov != 0) or m,   O = the above of u,
  *   w = w (1 - lr weight_decay) - lr scale O
  * lr is multiplied by *d_lr when that is not NULL (device memory: a captured step follows it).
- * scale 0 = sqrt(max(1, rows / cols)).  products 0 = 3.  Workspace as above.  w, g and m must not
+ * scale 0 = sqrt(max(1, rows / cols)), the factor of a weight stored [outputs][inputs]; one stored
+ * [inputs][outputs], as W_enc, takes sqrt(max(1, cols / rows)), given as scale.  products 0 = 3.  Workspace as above.  w, g and m must not
  * overlap. */
 int cfp_muon_update(float* d_w, const float* d_g, float* d_momentum, int64_t ld,
                     int64_t batch_stride, int batch, int rows, int cols, const float* d_lr, float lr,

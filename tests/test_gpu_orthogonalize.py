@@ -337,3 +337,17 @@ def test_fewer_bits_only_when_asked_for(pkg, cuda, dtype, batch, rows, cols):
     got = pkg.policy.orthogonalize(g)
     assert off(got, want) <= once + 2 * (5e-6 + 2.0 ** -21 * np.sqrt(max(rows, cols))), (off(got, want), once)
     assert torch.equal(got, pkg.policy.orthogonalize(g, products=3))
+
+
+@pytest.mark.parametrize("outputs,inputs", [(300, 80), (80, 300), (843, 256)])
+def test_default_scale_is_that_of_outputs_by_inputs(pkg, cuda, outputs, inputs):
+    """The step of a weight stored the other way round is the transposed one, its factor given."""
+    torch = _torch()
+    w, g, m = (gradient(cuda, 1, outputs, inputs, seed=50 + k, size=0.1 if k == 0 else 1e-3) for k in range(3))
+    w2, g2, m2 = (t.transpose(1, 2).contiguous() for t in (w, g, m))
+    want, _, step = muon_reference(w, g, m, 0.1, 0.95, True, 0.0, max(1.0, outputs / inputs) ** 0.5)
+    pkg.policy.muon_update(w, g, m, 0.1)
+    pkg.policy.muon_update(w2, g2, m2, 0.1, scale=max(1.0, outputs / inputs) ** 0.5)
+    bound = tolerance("f32", 3, w.shape) * step.norm() + 3 * 2.0 ** -24 * want.norm()
+    assert (w.double().cpu() - want).norm() <= bound
+    assert (w2.transpose(1, 2).double().cpu() - want).norm() <= bound
