@@ -185,6 +185,14 @@ struct Work {
     int mp, np, ldm, ldn;
 };
 
+// kScaleX / (|u| + eps) from the sum of squares, in 64 bits: the reciprocal of a norm below 3e-36 is
+// past fp32.  0 for a zero matrix without eps.  An infinity among the entries makes it NaN, as NaN
+// does: every entry of X then is, not only that one (inf * 0).
+__device__ __forceinline__ double scale_of(double squares, float eps) {
+    const double norm = sqrt(squares) + (double)eps;
+    return norm == 0.0 ? 0.0 : isinf(squares) ? (double)NAN : (double)kScaleX / norm;
+}
+
 // Second pass: X = u / (|u| + eps) times kScaleX in both orders, zeros in the padding.  A thread
 // takes four consecutive entries of four rows of a 64 x 64 tile, then of its transpose.
 template <int P>
@@ -217,9 +225,7 @@ __global__ __launch_bounds__(256) void k_ortho_load(InArgs a, Work w, int tall) 
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = s;
     __syncthreads();
-    // in 64 bits: the reciprocal of a norm below 3e-36 is past fp32
-    const double norm = sqrt((ws[0] + ws[1]) + (ws[2] + ws[3])) + (double)a.eps;
-    const double inv = norm == 0.0 ? 0.0 : (double)kScaleX / norm;
+    const double inv = scale_of((ws[0] + ws[1]) + (ws[2] + ws[3]), a.eps);
     _Float16* d1 = tall ? w.y[0] + (size_t)bt * w.np * w.ldm : w.x + (size_t)bt * w.mp * w.ldn;
     _Float16* d2 = tall ? w.x + (size_t)bt * w.mp * w.ldn : w.y[0] + (size_t)bt * w.np * w.ldm;
     const int ld1 = tall ? w.ldm : w.ldn, ld2 = tall ? w.ldn : w.ldm;
@@ -1111,11 +1117,10 @@ __global__ __launch_bounds__(64 * kSmallWaves) void k_ortho_small(SmallArgs g) {
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) ws[wave] = sum;
     __syncthreads();
-    double norm = 0.0;
+    double squares = 0.0;
 #pragma unroll
-    for (int w = 0; w < kSmallWaves; w++) norm += ws[w];
-    norm = sqrt(norm) + (double)in.eps;
-    const double inv = norm == 0.0 ? 0.0 : (double)kScaleX / norm;
+    for (int w = 0; w < kSmallWaves; w++) squares += ws[w];
+    const double inv = scale_of(squares, in.eps);
 #pragma unroll
     for (int b = 0; b < 2; b++)
 #pragma unroll

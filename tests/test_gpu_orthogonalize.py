@@ -351,3 +351,18 @@ def test_default_scale_is_that_of_outputs_by_inputs(pkg, cuda, outputs, inputs):
     bound = tolerance("f32", 3, w.shape) * step.norm() + 3 * 2.0 ** -24 * want.norm()
     assert (w.double().cpu() - want).norm() <= bound
     assert (w2.transpose(1, 2).double().cpu() - want).norm() <= bound
+
+
+@pytest.mark.parametrize("steps", [0, 1, 5])
+@pytest.mark.parametrize("rows,cols", [(30, 50), (300, 90)])
+def test_nan_and_infinity_take_the_whole_matrix(pkg, cuda, rows, cols, steps):
+    """At any number of steps, none among them; the batch's other matrices keep their values."""
+    torch = _torch()
+    base = gradient(cuda, 3, rows, cols, seed=8)
+    want = pkg.policy.orthogonalize(base, steps=steps)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        g = base.clone()
+        g[1, rows - 1, 3] = bad
+        got = pkg.policy.orthogonalize(g, steps=steps)
+        assert got[1].isnan().all() and torch.equal(got[::2], want[::2])
+    assert pkg.policy.orthogonalize(base, steps=steps, eps=float("inf")).eq(0).all()
