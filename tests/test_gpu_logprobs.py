@@ -610,3 +610,19 @@ def test_long_rows_keep_their_sums(pkg, cuda, dtype, rows, vocab):
     assert torch.equal(got.top_ids[:, 0], tok) and torch.equal(got.top_logprobs[:, 0], got.logprobs)
     del x
     torch.cuda.empty_cache()
+
+
+def test_sizes_past_the_library_counts_are_refused(pkg, cuda):
+    """2^32 + 43 columns are not 43, nor as many matrix columns 43."""
+    torch = _torch()
+    torch.cuda.empty_cache()
+    x = torch.empty((1, (1 << 32) + 43), dtype=torch.float16, device=cuda)
+    tok = torch.zeros(1, dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="logits: at most"):
+        pkg.policy.token_logprobs(x, tok)
+    with pytest.raises(ValueError, match="logits: at most"):
+        pkg.policy.token_logprobs_backward(x, tok, torch.zeros(1, 3, device=cuda))
+    with pytest.raises(ValueError, match="g: at most"):
+        pkg.policy.orthogonalize(x, out=x)
+    del x
+    torch.cuda.empty_cache()
