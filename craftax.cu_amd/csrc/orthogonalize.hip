@@ -15,7 +15,7 @@
 // accumulation, scaled by a power of two so that the range in use sits in the middle of fp16's
 // (singular values stay under 1.21 with the standard coefficients; X is held times 2^10, A and
 // B times 2^8, so |X| < 64 and |A|, |B| < 256 for other ones):
-//   P = 3  every matrix is a pair hi + lo of fp16 numbers (22 bits, or to 2^-35 of 1) and a
+//   P = 3  every matrix is a pair hi + lo of fp16 numbers (22 bits, X at best to 2^-35) and a
 //          product is hi hi + hi lo + lo hi: what is left out, lo lo, is below 2^-22 of a
 //          product.  Error against 64 bits about 1e-6 of the result's norm, as fp32 has.
 //          What every input type gets unless the caller asks for less.

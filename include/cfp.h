@@ -451,13 +451,15 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
  * it: X = G / (|G|_F + eps), then `steps` (0..16) times, with the step's a, b, c,
  *   A = X X^T,  B = b A + c A A,  X = a X + B X      (on the shorter side of G)
  * d_g and d_out: `batch` matrices rows x cols (1..65536 each) of element type `dtype`, row
- * strides ld / ld_out and matrix strides batch_stride / out_batch_stride in elements (any for a
- * batch of one); d_out may be d_g with the same strides, any other overlap is an error.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315) for
- * every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
+ * strides ld / ld_out and matrix strides batch_stride / out_batch_stride in elements (at least
+ * (rows - 1) ld + cols; any for a batch of one); d_out may be d_g with the same strides or lie
+ * beside it, an overlap is an error.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315)
+ * for every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
  * products: 3 (or 0) = three fp16 matrix products per product (1e-6 of the result's norm from the
- * 64-bit result, as fp32 has), 1 = one (up to 2e-3, in a third of the time).  Sums are fp32, the
- * norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes all
- * of it NaN.
+ * 64-bit result, as fp32 has), 1 = one (up to 2e-3, in a third of the time).  Entries of X are held
+ * to 2^-35 at best: a |G| far below eps, whose result is small, leaves an error of up to 2e-8
+ * sqrt(rows cols) after five standard steps.  Sums are fp32, the norm is 64-bit.  A zero matrix
+ * gives zeros; NaN or infinity in a matrix makes all of it NaN.
  * d_work: cfp_orthogonalize_workspace(batch, rows, cols, products) bytes (products 1 or 3),
  * 256-byte aligned (may be NULL where that is 0: matrices that fit into one workgroup); calls that
  * may overlap need one each. */
@@ -472,8 +474,8 @@ int cfp_orthogonalize(const void* d_g, int dtype, int64_t ld, int64_t batch_stri
  *   w = w (1 - lr weight_decay) - lr scale O
  * lr is multiplied by *d_lr when that is not NULL (device memory: a captured step follows it).
  * scale 0 = sqrt(max(1, rows / cols)), the factor of a weight stored [outputs][inputs]; one stored
- * [inputs][outputs], as W_enc, takes sqrt(max(1, cols / rows)), given as scale.  products 0 = 3.  Workspace as above.  w, g and m must not
- * overlap. */
+ * [inputs][outputs], as W_enc, takes sqrt(max(1, cols / rows)), given as scale.  products 0 = 3.
+ * Workspace as above.  w, g and m must not overlap. */
 int cfp_muon_update(float* d_w, const float* d_g, float* d_momentum, int64_t ld,
                     int64_t batch_stride, int batch, int rows, int cols, const float* d_lr, float lr,
                     float momentum, int nesterov, float weight_decay, float scale, int steps,

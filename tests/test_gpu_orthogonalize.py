@@ -366,3 +366,19 @@ def test_nan_and_infinity_take_the_whole_matrix(pkg, cuda, rows, cols, steps):
         got = pkg.policy.orthogonalize(g, steps=steps)
         assert got[1].isnan().all() and torch.equal(got[::2], want[::2])
     assert pkg.policy.orthogonalize(base, steps=steps, eps=float("inf")).eq(0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(48, 80), (256, 300), (900, 700)])
+@pytest.mark.parametrize("below", [1.0, 1e3, 1e6, 1e9])
+def test_norms_far_below_eps(pkg, cuda, rows, cols, below):
+    """|G| = eps / below.  X is held to 2^-35 an entry (half a denormal step of fp16, times 2^10), so
+    every step leaves up to 2^-35 sqrt(rows cols), which the remaining ones amplify by 3.4445 each at
+    most: 683 times that (the sum of the powers 1 .. 5).  A and B are held to 2^-33: (4.775 + 1) 2^-33 m
+    of X a step."""
+    g = gradient(cuda, 1, rows, cols, seed=rows)
+    g *= 1e-7 / below / g.norm()
+    want = reference(g)
+    got = pkg.policy.orthogonalize(g)
+    m = min(rows, cols)
+    bound = (tolerance("f32", 3, g.shape) + 5 * 5.775 / 3.4445 * 2.0 ** -33 * m) * want.norm() + 683 * 2.0 ** -35 * (rows * cols) ** 0.5
+    assert (got.double().cpu() - want).norm() <= bound
