@@ -20,8 +20,9 @@ def hipcc_path():
 
 # Kernels that wait for loads they issue from inline assembly with explicit
 # `s_waitcnt vmcnt(N)`, N = the number of younger vector-memory operations the
-# source issues: the fused fp32 forward (both tile sizes) and the reverse MinGRU sweep.
-COUNTED_WAIT_KERNELS = ("k_policy_forwardI", "k_policy_forward_t16I", "k_gru_reverseI")
+# source issues: the fused fp32 forward (both tile sizes), the reverse MinGRU sweep, and the
+# Newton-Schulz products whose copies to LDS run through a ring.
+COUNTED_WAIT_KERNELS = ("k_policy_forwardI", "k_policy_forward_t16I", "k_gru_reverseI", "k_ortho_mulI", "k_ortho_pairI")
 
 
 def check_no_scratch(remarks):
@@ -42,13 +43,15 @@ def check_no_scratch(remarks):
 # the operations the source issues between a load and its use; how many wavefronts share a
 # SIMD decides how far ahead those loads have to be issued (the forward kernels are written
 # for one, respectively two, wavefronts per SIMD; the sweep for at least four, its
-# __launch_bounds__), and a jump in registers is how a compiler change that re-orders or
+# __launch_bounds__; the Newton-Schulz products for one or two, as their LDS rings fit), and a jump in registers is how a compiler change that re-orders or
 # duplicates those loads shows first.  (kernel name part, VGPRs allowed, AGPRs allowed,
 # occupancy [waves/SIMD] lowest, highest)
 COUNTED_WAIT_BUDGET = (
     ("k_policy_forwardI", 256, 160, 1, 1),
     ("k_policy_forward_t16I", 192, 0, 2, 2),
     ("k_gru_reverseI", 128, 0, 4, 8),
+    ("k_ortho_mulI", 192, 256, 1, 2),
+    ("k_ortho_pairI", 128, 64, 1, 2),
 )
 
 

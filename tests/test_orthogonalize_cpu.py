@@ -108,3 +108,23 @@ def test_muon_refuses_a_scale_below_zero(pkg, scale):
     far = [C.c_void_p(0x10000 + k * BIG) for k in range(3)]
     assert lib.cfp_muon_update(*far, 64, 4096, 1, 64, 64, None, 0.1, 0.9, 1, 0.0, scale, 5, None, 1e-7, 0, P, BIG, None) != 0
     assert b"scale" in lib.cfp_last_error()
+
+
+def test_build_refuses_products_that_spill_or_outgrow_their_budget():
+    """k_ortho_mul and k_ortho_pair wait for counted copies."""
+    import __graft_entry__ as entry
+    build = entry._load_build_module()
+
+    def remarks(name, vgprs=80, agprs=32, scratch=0, occupancy=2):
+        return "\n".join(f"x.hip:1:1: remark: {l} [-Rpass-analysis=kernel-resource-usage]" for l in (
+            f"Function Name: _ZN3cfp12_GLOBAL__N_1{len(name)}{name}ILi3ELi0ELi1EEEv", f"    VGPRs: {vgprs}", f"    AGPRs: {agprs}",
+            f"    ScratchSize [bytes/lane]: {scratch}", f"    Occupancy [waves/SIMD]: {occupancy}"))
+
+    for name in ("k_ortho_mul", "k_ortho_pair"):
+        build.check_no_scratch(remarks(name))
+        build.check_counted_wait_budget(remarks(name))
+        with pytest.raises(RuntimeError, match=name):
+            build.check_no_scratch(remarks(name, scratch=16))
+        for kw in (dict(vgprs=200), dict(agprs=300), dict(occupancy=0), dict(occupancy=4)):
+            with pytest.raises(RuntimeError, match=name):
+                build.check_counted_wait_budget(remarks(name, **kw))
