@@ -382,3 +382,55 @@ def test_norms_far_below_eps(pkg, cuda, rows, cols, below):
     m = min(rows, cols)
     bound = (tolerance("f32", 3, g.shape) + 5 * 5.775 / 3.4445 * 2.0 ** -33 * m) * want.norm() + 683 * 2.0 ** -35 * (rows * cols) ** 0.5
     assert (got.double().cpu() - want).norm() <= bound
+
+
+def in_the_formats(g, products, steps=5, eps=1e-7):
+    """The definition with the kernels' number formats, on the CPU: X, A and B as fp16 (scaled by 2^10,
+    2^8, 2^8) or hi + lo pairs of it, products hi hi (+ hi lo + lo hi), sums in float32 of another order."""
+    torch = _torch()
+
+    def pair(v, scale):
+        v = (v * scale).float()
+        hi = v.half().float()
+        return hi / scale, (v - hi).half().float() / scale
+
+    def product(l, r):
+        out = l[0] @ r[0]
+        return out if products == 1 else out + (l[0] @ r[1] + l[1] @ r[0])
+
+    x = g.double().cpu()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.transpose(-1, -2) if tall else x
+    x = (x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)).float()
+    turned = lambda p: tuple(t.transpose(-1, -2).contiguous() for t in p)
+    for _ in range(steps):
+        X = pair(x, 1024.0)
+        A = pair(product(X, turned(X)), 256.0)
+        a = A[0] if products == 1 else A[0] + A[1]
+        B = pair(QUINTIC[1] * a + QUINTIC[2] * product(A, A), 256.0)
+        x = QUINTIC[0] * (X[0] + X[1]) + product(B, X)
+    return (x.transpose(-1, -2) if tall else x).double()
+
+
+@pytest.mark.parametrize("products", [1, 3])
+@pytest.mark.parametrize("rows,cols,fall", [(200, 320, 0.0), (200, 320, 1.0), (200, 320, 3.0), (60, 90, 0.5), (843, 256, 0.5),
+                                            (700, 900, 0.5), (128, 512, 0.5), (1, 300, 0.0), (150, 400, None)])
+def test_errors_are_those_of_the_formats(pkg, cuda, products, rows, cols, fall):
+    """Against 64 bits the kernels are off by what their number formats leave, measured by the same
+    roundings on the CPU rather than bounded.  One product: fp16's roundings (2^-12) are the same on
+    both sides but where sums in fp32, off by up to 2^-24 sqrt(K) of themselves, fall on the other
+    side of a border; that happens to a part 2^-13 sqrt(K) of them and moves those by a step, 12
+    times a rounding's square: sqrt(12 * 2^-13 * sqrt(1024)) = 0.22 of the roundings' norm, taken as
+    half of it.  Three: the 2^-23 of the pairs and the fp32 sums weigh alike, and sums are formed in
+    another order, sixteen terms at a time here: taken as up to three times the norm.  fall None: one
+    direction only."""
+    torch = _torch()
+    if fall is None:
+        gen = torch.Generator().manual_seed(3)
+        g = (torch.randn(1, rows, 1, generator=gen) * torch.randn(1, 1, cols, generator=gen)).to(cuda)
+    else:
+        g = gradient(cuda, 1, rows, cols, seed=rows + 5, fall=fall)
+    want = reference(g)
+    there = (in_the_formats(g, products) - want).norm()
+    here = (pkg.policy.orthogonalize(g, products=products).double().cpu() - want).norm()
+    assert here <= (1.5 if products == 1 else 3.0) * there + 2.0 ** -24 * want.norm(), (here / want.norm(), there / want.norm())
