@@ -269,6 +269,7 @@ struct LpArgs {
     int64_t ld_mask;       // 0: one mask for all rows
     float* lp;
     float* ent;            // or null
+    int row0;              // of this launch (k_logprobs_short)
     int top;
     int32_t* ids;
     float* top_lp;
@@ -354,92 +355,90 @@ template <typename T, int L, int Q, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_short(LpArgs a) {
     constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
-    const int per = 256 / L;
-    for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
-        const bool live = row0 + (int)threadIdx.x / L < a.rows;
-        const int r = live ? (int)row0 + (int)threadIdx.x / L : a.rows - 1;
-        const int tok = a.tok[r];
-        const float xt = token_logit<T>(a, r, tok);
-        float v[Q][N];
-        int first[Q];
-        load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
-                                  a.vocab, sub, v, first);
-        Sums z;
+    const unsigned row = (unsigned)a.row0 + blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool live = row < (unsigned)a.rows;
+    const int r = live ? (int)row : a.rows - 1;
+    const int tok = a.tok[r];
+    const float xt = token_logit<T>(a, r, tok);
+    float v[Q][N];
+    int first[Q];
+    load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
+                              a.vocab, sub, v, first);
+    Sums z;
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+        for (int j = 0; j < N; j++) z.m = fmaxf(z.m, v[q][j]);
+    z.m = max_lanes<L>(z.m);
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+        for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
+    z.s = sum_lanes<L>(z.s);
+    z.u = sum_lanes<L>(z.u);
+    if (live && sub == 0) write_row(a, r, z, tok, xt);
+    if (a.top == 0) return;
+    // Alternatives: the maximum of the row, then the lowest index that holds it, `top` times; lane
+    // k (then k - L) keeps number k, and all are written together.  16-bit entries and their index
+    // make one 32-bit key (rows have at most 1024 of them): 262 144 x 43 fp16 with 20 alternatives
+    // take 85 us, 150 with value and index apart, as fp32 has them (111).
+    constexpr int SLOTS = kMaxTop > L ? kMaxTop / L : 1;
+    if constexpr (sizeof(T) == 2) {
+        unsigned key[Q][N], kept[SLOTS] = {};
 #pragma unroll
         for (int q = 0; q < Q; q++)
 #pragma unroll
-            for (int j = 0; j < N; j++) z.m = fmaxf(z.m, v[q][j]);
-        z.m = max_lanes<L>(z.m);
-#pragma unroll
-        for (int q = 0; q < Q; q++)
-#pragma unroll
-            for (int j = 0; j < N; j++) add_entry(z, v[q][j]);
-        z.s = sum_lanes<L>(z.s);
-        z.u = sum_lanes<L>(z.u);
-        if (live && sub == 0) write_row(a, r, z, tok, xt);
-        if (a.top == 0) continue;
-        // Alternatives: the maximum of the row, then the lowest index that holds it, `top` times; lane
-        // k (then k - L) keeps number k, and all are written together.  16-bit entries and their index
-        // make one 32-bit key (rows have at most 1024 of them): 262 144 x 43 fp16 with 20 alternatives
-        // take 85 us, 150 with value and index apart, as fp32 has them (111).
-        constexpr int SLOTS = kMaxTop > L ? kMaxTop / L : 1;
-        if constexpr (sizeof(T) == 2) {
-            unsigned key[Q][N], kept[SLOTS] = {};
+            for (int j = 0; j < N; j++) key[q][j] = v[q][j] > -INFINITY ? short_key<T>(v[q][j], first[q] + j) : 0u;
+        for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
+            unsigned best = 0;
 #pragma unroll
             for (int q = 0; q < Q; q++)
 #pragma unroll
-                for (int j = 0; j < N; j++) key[q][j] = v[q][j] > -INFINITY ? short_key<T>(v[q][j], first[q] + j) : 0u;
-            for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
-                unsigned best = 0;
-#pragma unroll
-                for (int q = 0; q < Q; q++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) best = max(best, key[q][j]);
-                best = max(best, xor_lane<1>(best));
-                best = max(best, xor_lane<2>(best));
-                best = max(best, xor_lane<4>(best));
-                best = max(best, xor_lane<8>(best));
-                if (L == 64) {
-                    best = max(best, xor_lane<16>(best));
-                    best = max(best, xor_lane<32>(best));
-                }
-#pragma unroll
-                for (int q = 0; q < Q; q++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) key[q][j] = key[q][j] == best ? 0u : key[q][j];
-#pragma unroll
-                for (int t = 0; t < SLOTS; t++) kept[t] = k == t * L + sub ? best : kept[t];
+                for (int j = 0; j < N; j++) best = max(best, key[q][j]);
+            best = max(best, xor_lane<1>(best));
+            best = max(best, xor_lane<2>(best));
+            best = max(best, xor_lane<4>(best));
+            best = max(best, xor_lane<8>(best));
+            if (L == 64) {
+                best = max(best, xor_lane<16>(best));
+                best = max(best, xor_lane<32>(best));
             }
 #pragma unroll
-            for (int t = 0; t < SLOTS; t++)
-                if (live && t * L + sub < a.top)
-                    write_top(a, r, z, t * L + sub, kept[t] ? key_of(short_value<T>(kept[t]), 0xffff - (int)(kept[t] & 0xffffu)) : 0);
-            continue;
-        }
-        uint64_t kept[SLOTS] = {};
-        for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
-            float bv = -INFINITY;
-            int bi = INT_MAX;
-#pragma unroll
             for (int q = 0; q < Q; q++)
 #pragma unroll
-                for (int j = 0; j < N; j++)   // ascending index: ties keep the first
-                    if (v[q][j] > bv) { bv = v[q][j]; bi = first[q] + j; }
-            const float m = max_lanes<L>(bv);
-            bi = min_lanes<L>(bv == m ? bi : INT_MAX);
+                for (int j = 0; j < N; j++) key[q][j] = key[q][j] == best ? 0u : key[q][j];
 #pragma unroll
-            for (int q = 0; q < Q; q++)
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (first[q] + j == bi) v[q][j] = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < SLOTS; t++)
-                if (k == t * L + sub) kept[t] = bi == INT_MAX ? 0 : key_of(m, bi);
+            for (int t = 0; t < SLOTS; t++) kept[t] = k == t * L + sub ? best : kept[t];
         }
 #pragma unroll
         for (int t = 0; t < SLOTS; t++)
-            if (live && t * L + sub < a.top) write_top(a, r, z, t * L + sub, kept[t]);
+            if (live && t * L + sub < a.top)
+                write_top(a, r, z, t * L + sub, kept[t] ? key_of(short_value<T>(kept[t]), 0xffff - (int)(kept[t] & 0xffffu)) : 0);
+        return;
     }
+    uint64_t kept[SLOTS] = {};
+    for (int k = 0; k < a.top; k++) {   // wave-uniform trip count
+        float bv = -INFINITY;
+        int bi = INT_MAX;
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++)   // ascending index: ties keep the first
+                if (v[q][j] > bv) { bv = v[q][j]; bi = first[q] + j; }
+        const float m = max_lanes<L>(bv);
+        bi = min_lanes<L>(bv == m ? bi : INT_MAX);
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (first[q] + j == bi) v[q][j] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < SLOTS; t++)
+            if (k == t * L + sub) kept[t] = bi == INT_MAX ? 0 : key_of(m, bi);
+    }
+#pragma unroll
+    for (int t = 0; t < SLOTS; t++)
+        if (live && t * L + sub < a.top) write_top(a, r, z, t * L + sub, kept[t]);
 }
 
 // ---- short rows, many of them: one thread a row ------------------------------------------
@@ -464,11 +463,11 @@ struct RowVectors {
         first = min((q - row * per_row) * N, vocab - N);
     }
 };
-// Rows [r0, r0 + kRowsThreads) of x as fp32 into LDS, -inf where masked; all of a thread's loads in
-// flight together (at most PASSES; per_row of them).
+// `rows` rows from x on (kRowsThreads at most) as fp32 into LDS, -inf where masked; all of a thread's
+// loads in flight together (at most PASSES; per_row of them).
 template <typename T, int PASSES, bool MASK>
-__device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t* mask, int64_t ld_mask, int64_t r0, int rows,
-                                           int vocab, float* stage) {
+__device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t* mask, int64_t ld_mask, int rows, int vocab,
+                                           float* stage) {
     constexpr int N = Vec<T>::N;
     const RowVectors<N> rv(vocab);
     Vec<T> v[PASSES];
@@ -477,16 +476,16 @@ __device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t
     for (int p = 0; p < PASSES; p++) {
         int r, i;
         rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
-        if (p >= rv.per_row || r0 + r >= rows) continue;
-        v[p] = load_vec(x + (size_t)(r0 + r) * ld + i);
-        if (MASK) __builtin_memcpy(mk[p], mask + (size_t)(r0 + r) * ld_mask + i, N);
+        if (p >= rv.per_row || r >= rows) continue;
+        v[p] = load_vec(x + (size_t)r * ld + i);
+        if (MASK) __builtin_memcpy(mk[p], mask + (size_t)r * ld_mask + i, N);
     }
     const int pitch = rows_pitch(vocab);
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         int r, i;
         rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
-        if (p >= rv.per_row || r0 + r >= rows) continue;
+        if (p >= rv.per_row || r >= rows) continue;
 #pragma unroll
         for (int j = 0; j < N; j++) stage[r * pitch + i + j] = MASK && mk[p][j] == 0 ? -INFINITY : to_f32(v[p].v[j]);
     }
@@ -494,21 +493,20 @@ __device__ __forceinline__ void stage_rows(const T* x, int64_t ld, const uint8_t
 template <typename T, int PASSES, bool MASK>
 __global__ __launch_bounds__(kRowsThreads) void k_logprobs_rows(LpArgs a) {
     extern __shared__ float stage[];
-    for (int64_t r0 = (int64_t)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int64_t)gridDim.x * kRowsThreads) {
-        const int64_t row = r0 + (int)threadIdx.x;
-        stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
-        const int tok = row < a.rows ? a.tok[row] : -1;
-        __syncthreads();
-        if (row < a.rows) {
-            const float* x = stage + threadIdx.x * rows_pitch(a.vocab);
-            Sums z;
+    const int r0 = (int)blockIdx.x * kRowsThreads, row = r0 + (int)threadIdx.x, here = min(kRowsThreads, a.rows - r0);
+    const bool live = row < a.rows;
+    stage_rows<T, PASSES, MASK>((const T*)a.x + r0 * a.ld, a.ld, MASK ? a.mask + r0 * a.ld_mask : nullptr, a.ld_mask, here,
+                                a.vocab, stage);
+    const int tok = live ? a.tok[row] : -1;
+    __syncthreads();
+    if (live) {
+        const float* x = stage + threadIdx.x * rows_pitch(a.vocab);
+        Sums z;
 #pragma unroll 4
-            for (int i = 0; i < a.vocab; i++) z.m = fmaxf(z.m, x[i]);
+        for (int i = 0; i < a.vocab; i++) z.m = fmaxf(z.m, x[i]);
 #pragma unroll 4
-            for (int i = 0; i < a.vocab; i++) add_entry(z, x[i]);
-            write_row(a, (int)row, z, tok, tok >= 0 && tok < a.vocab ? x[tok] : -INFINITY);
-        }
-        __syncthreads();
+        for (int i = 0; i < a.vocab; i++) add_entry(z, x[i]);
+        write_row(a, row, z, tok, tok >= 0 && tok < a.vocab ? x[tok] : -INFINITY);
     }
 }
 
@@ -724,6 +722,7 @@ struct LpGradArgs {
     void* dx;
     int64_t ld_dx;
     int splits, chunk;
+    int row0;              // of this launch (k_logprobs_grad_short, k_logprobs_grad)
 };
 // What a row's entries share.
 struct RowGrad {
@@ -764,52 +763,50 @@ template <typename T, int L, int Q, bool MASK>
 __global__ __launch_bounds__(256) void k_logprobs_grad_short(LpGradArgs a) {
     constexpr int N = Vec<T>::N;
     const int sub = threadIdx.x % L;
-    const int per = 256 / L;
-    for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += (int64_t)gridDim.x * per) {
-        const bool live = row0 + (int)threadIdx.x / L < a.rows;
-        const int r = live ? (int)row0 + (int)threadIdx.x / L : a.rows - 1;
-        float v[Q][N], d[Q][N];
-        int first[Q];
-        load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
-                                  a.vocab, sub, v, first);
+    const unsigned row = (unsigned)a.row0 + blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool live = row < (unsigned)a.rows;
+    const int r = live ? (int)row : a.rows - 1;
+    float v[Q][N], d[Q][N];
+    int first[Q];
+    load_short<T, L, Q, MASK>((const T*)a.x + (size_t)r * a.ld, MASK ? a.mask + (size_t)r * a.ld_mask : nullptr,
+                              a.vocab, sub, v, first);
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+        for (int j = 0; j < N; j++) d[q][j] = 0.0f;
+    // the named entries: whose lane holds an allowed one takes its gradient
+    float weight = 0.0f;
+    for (int k = 0; k <= a.top; k++) {
+        if (k == 0 && !a.g_lp) continue;
+        const int i = k == 0 ? a.tok[r] : a.ids[(size_t)r * a.top + k - 1];
+        const float g = k == 0 ? a.g_lp[r] : a.g_top[(size_t)r * a.top + k - 1];
+        if (i >= a.vocab && sub == 0) weight = NAN;
 #pragma unroll
         for (int q = 0; q < Q; q++)
 #pragma unroll
-            for (int j = 0; j < N; j++) d[q][j] = 0.0f;
-        // the named entries: whose lane holds an allowed one takes its gradient
-        float weight = 0.0f;
-        for (int k = 0; k <= a.top; k++) {
-            if (k == 0 && !a.g_lp) continue;
-            const int i = k == 0 ? a.tok[r] : a.ids[(size_t)r * a.top + k - 1];
-            const float g = k == 0 ? a.g_lp[r] : a.g_top[(size_t)r * a.top + k - 1];
-            if (i >= a.vocab && sub == 0) weight = NAN;
+            for (int j = 0; j < N; j++)
+                if (first[q] + j == i && !(v[q][j] == -INFINITY)) { d[q][j] += g; weight += g; }
+    }
+    RowGrad rg;
+    row_grad(a, r, sum_lanes<L>(weight), rg);
+    T* dx = (T*)a.dx + (size_t)r * a.ld_dx;
 #pragma unroll
-            for (int q = 0; q < Q; q++)
+    for (int q = 0; q < Q; q++) {
+        // every load of this row was used above: the row may be overwritten in place.  Each
+        // entry is stored by the lane that it counts for.
+        const int i = (q * L + sub) * N;
+        Vec<T> out;
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (first[q] + j == i && !(v[q][j] == -INFINITY)) { d[q][j] += g; weight += g; }
+        for (int j = 0; j < N; j++) {
+            const bool on = !rg.none && !(v[q][j] == -INFINITY);
+            out.v[j] = (T)(on ? rg.at(v[q][j]) + d[q][j] : 0.0f);
         }
-        RowGrad rg;
-        row_grad(a, r, sum_lanes<L>(weight), rg);
-        T* dx = (T*)a.dx + (size_t)r * a.ld_dx;
+        if (!live) continue;
+        if (i + N <= a.vocab) store_vec(dx + i, out);
+        else
 #pragma unroll
-        for (int q = 0; q < Q; q++) {
-            // every load of this row was used above: the row may be overwritten in place.  Each
-            // entry is stored by the lane that it counts for.
-            const int i = (q * L + sub) * N;
-            Vec<T> out;
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const bool on = !rg.none && !(v[q][j] == -INFINITY);
-                out.v[j] = (T)(on ? rg.at(v[q][j]) + d[q][j] : 0.0f);
-            }
-            if (!live) continue;
-            if (i + N <= a.vocab) store_vec(dx + i, out);
-            else
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (first[q] + j >= i && first[q] + j < a.vocab) dx[first[q] + j] = out.v[j];
-        }
+            for (int j = 0; j < N; j++)
+                if (first[q] + j >= i && first[q] + j < a.vocab) dx[first[q] + j] = out.v[j];
     }
 }
 
@@ -819,51 +816,49 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
     extern __shared__ float stage[];
     constexpr int N = Vec<T>::N;
     const int pitch = rows_pitch(a.vocab);
-    for (int64_t r0 = (int64_t)blockIdx.x * kRowsThreads; r0 < a.rows; r0 += (int64_t)gridDim.x * kRowsThreads) {
-        const int64_t row = r0 + (int)threadIdx.x;
-        stage_rows<T, PASSES, MASK>((const T*)a.x, a.ld, a.mask, a.ld_mask, r0, a.rows, a.vocab, stage);
-        int tok = -1;
-        float g = 0.0f;
-        if (row < a.rows && a.g_lp) { tok = a.tok[row]; g = a.g_lp[row]; }
-        __syncthreads();
-        if (row < a.rows) {
-            float* x = stage + threadIdx.x * pitch;
-            const bool hit = tok >= 0 && tok < a.vocab && !(x[tok] == -INFINITY);
-            RowGrad rg;
-            row_grad(a, (int)row, tok >= a.vocab ? NAN : hit ? g : 0.0f, rg);
+    const int r0 = (int)blockIdx.x * kRowsThreads, row = r0 + (int)threadIdx.x, here = min(kRowsThreads, a.rows - r0);
+    const bool live = row < a.rows;
+    stage_rows<T, PASSES, MASK>((const T*)a.x + r0 * a.ld, a.ld, MASK ? a.mask + r0 * a.ld_mask : nullptr, a.ld_mask, here,
+                                a.vocab, stage);
+    int tok = -1;
+    float g = 0.0f;
+    if (live && a.g_lp) { tok = a.tok[row]; g = a.g_lp[row]; }
+    __syncthreads();
+    if (live) {
+        float* x = stage + threadIdx.x * pitch;
+        const bool hit = tok >= 0 && tok < a.vocab && !(x[tok] == -INFINITY);
+        RowGrad rg;
+        row_grad(a, row, tok >= a.vocab ? NAN : hit ? g : 0.0f, rg);
 #pragma unroll 4
-            for (int i = 0; i < a.vocab; i++) {
-                const float v = x[i];
-                x[i] = rg.none || v == -INFINITY ? 0.0f : rg.at(v) + (i == tok ? g : 0.0f);
-            }
+        for (int i = 0; i < a.vocab; i++) {
+            const float v = x[i];
+            x[i] = rg.none || v == -INFINITY ? 0.0f : rg.at(v) + (i == tok ? g : 0.0f);
         }
-        __syncthreads();
-        const int here = (int)min((int64_t)kRowsThreads, a.rows - r0) * pitch;
-        if (a.ld_dx == a.vocab && pitch == a.vocab && here % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
-            // rows without gaps, in memory and (odd widths) in LDS: one run of aligned vectors (r0 * pitch
-            // is a multiple of kRowsThreads)
-            T* dx = (T*)a.dx + (size_t)r0 * pitch;
+    }
+    __syncthreads();
+    T* dx = (T*)a.dx + r0 * a.ld_dx;
+    if (a.ld_dx == a.vocab && pitch == a.vocab && here * pitch % N == 0 && (reinterpret_cast<uintptr_t>(a.dx) & 15u) == 0) {
+        // rows without gaps, in memory and (odd widths) in LDS: one run of aligned vectors (r0 is a
+        // multiple of kRowsThreads)
 #pragma unroll 4
-            for (int e = (int)threadIdx.x * N; e < here; e += kRowsThreads * N) {
-                Vec<T> out;
+        for (int e = (int)threadIdx.x * N; e < here * pitch; e += kRowsThreads * N) {
+            Vec<T> out;
 #pragma unroll
-                for (int j = 0; j < N; j++) out.v[j] = (T)stage[e + j];
-                store_vec(dx + e, out);
-            }
-        } else {
-            const RowVectors<N> rv(a.vocab);
-#pragma unroll
-            for (int p = 0; p < PASSES; p++) {
-                int r, i;
-                rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
-                if (p >= rv.per_row || r0 + r >= a.rows) continue;
-                Vec<T> out;
-#pragma unroll
-                for (int j = 0; j < N; j++) out.v[j] = (T)stage[r * pitch + i + j];
-                store_vec((T*)a.dx + (size_t)(r0 + r) * a.ld_dx + i, out);   // repeated entries: the same values
-            }
+            for (int j = 0; j < N; j++) out.v[j] = (T)stage[e + j];
+            store_vec(dx + e, out);
         }
-        __syncthreads();
+    } else {
+        const RowVectors<N> rv(a.vocab);
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            int r, i;
+            rv.at(p * kRowsThreads + (int)threadIdx.x, r, i);
+            if (p >= rv.per_row || r >= here) continue;
+            Vec<T> out;
+#pragma unroll
+            for (int j = 0; j < N; j++) out.v[j] = (T)stage[r * pitch + i + j];
+            store_vec(dx + (size_t)r * a.ld_dx + i, out);   // repeated entries: the same values
+        }
     }
 }
 
@@ -872,65 +867,62 @@ __global__ __launch_bounds__(kRowsThreads) void k_logprobs_grad_rows(LpGradArgs 
 // before the first store, their values stored behind the last one (barriers on both sides).  The
 // barriers order one workgroup only, and every workgroup of a row reads all of its named logits:
 // where dx is x, a row has one workgroup (plan_grad), of kInPlaceThreads (bf16, in parts to another
-// array / in place by 256 / 512 / 1024 threads: 1 x 131 072 4 / 28 / 17 / 15 us, 128 x 131 072
-// 16 / 33 / 22 / 19, 2048 x 131 072 193 / 217 / 207 / 201, 4096 x 50 021 219 / 177 / 170 / 294,
-// 4096 x 4000 39 / 27 / 32 / 53).
+// array / in place by 256 / 512 / 1024 threads: 1 x 131 072 4 / 27 / 17 / 15 us, 128 x 131 072
+// 15 / 33 / 22 / 20, 2048 x 131 072 195 / 217 / 209 / 196, 4096 x 50 021 206 / 176 / 171 / 217,
+// 4096 x 4000 32 / 22 / 26 / 32).
 constexpr int kInPlaceThreads = 512;
 template <typename T, bool MASK, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_logprobs_grad(LpGradArgs a) {
     constexpr int N = Vec<T>::N, STRIDE = THREADS * N, TILE = STRIDE * kU;
-    const int64_t items = (int64_t)a.rows * a.splits;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int row = (int)(item / a.splits), split = (int)(item % a.splits);
-        const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
-        const T* x = (const T*)a.x + (size_t)row * a.ld;
-        const uint8_t* mask = MASK ? a.mask + (size_t)row * a.ld_mask : nullptr;
-        T* dx = (T*)a.dx + (size_t)row * a.ld_dx;
-        const int lane = threadIdx.x & 63;
-        // every wavefront holds all named entries, one a lane (top <= 32)
-        float g;
-        const int named = named_entry<T>(a, row, lane, g);
-        RowGrad rg;
-        row_grad(a, row, sum_lanes<64>(g), rg);
-        float patch = 0.0f;
-        const bool mine = threadIdx.x < 64 && named >= lo && named < hi && !rg.none;
-        if (threadIdx.x < 64) {
-            patch = mine ? rg.at(to_f32(x[named])) : 0.0f;
-            for (int j = 0; j <= a.top; j++)   // an index that is named twice gets both gradients
-                if (__builtin_amdgcn_readlane(named, j) == named)
-                    patch += lane_value(g, j);
-        }
-        __syncthreads();
-        int base = lo;
-        for (; base + TILE <= hi; base += TILE) {
-            const int i0 = base + (int)threadIdx.x * N;
-            Vec<T> raw[kU];
-            uint8_t mk[kU][N];
-#pragma unroll
-            for (int q = 0; q < kU; q++) {
-                raw[q] = load_vec(x + i0 + q * STRIDE);
-                if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
-            }
-#pragma unroll
-            for (int q = 0; q < kU; q++) {
-                Vec<T> out;
-#pragma unroll
-                for (int j = 0; j < N; j++) {
-                    const float xv = to_f32(raw[q].v[j]);
-                    const bool on = !rg.none && !(MASK && mk[q][j] == 0) && !(xv == -INFINITY);
-                    out.v[j] = (T)(on ? rg.at(xv) : 0.0f);
-                }
-                store_vec(dx + i0 + q * STRIDE, out);
-            }
-        }
-        for (int i = base + (int)threadIdx.x; i < hi; i += THREADS) {
-            const float xv = to_f32(x[i]);
-            const bool on = !rg.none && !(MASK && mask[i] == 0) && !(xv == -INFINITY);
-            dx[i] = (T)(on ? rg.at(xv) : 0.0f);
-        }
-        __syncthreads();
-        if (mine) dx[named] = (T)patch;
+    const int row = a.row0 + (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
+    const int lo = split * a.chunk, hi = lo + a.chunk < a.vocab ? lo + a.chunk : a.vocab;
+    const T* x = (const T*)a.x + (size_t)row * a.ld;
+    const uint8_t* mask = MASK ? a.mask + (size_t)row * a.ld_mask : nullptr;
+    T* dx = (T*)a.dx + (size_t)row * a.ld_dx;
+    const int lane = threadIdx.x & 63;
+    // every wavefront holds all named entries, one a lane (top <= 32)
+    float g;
+    const int named = named_entry<T>(a, row, lane, g);
+    RowGrad rg;
+    row_grad(a, row, sum_lanes<64>(g), rg);
+    float patch = 0.0f;
+    const bool mine = threadIdx.x < 64 && named >= lo && named < hi && !rg.none;
+    if (threadIdx.x < 64) {
+        patch = mine ? rg.at(to_f32(x[named])) : 0.0f;
+        for (int j = 0; j <= a.top; j++)   // an index that is named twice gets both gradients
+            if (__builtin_amdgcn_readlane(named, j) == named)
+                patch += lane_value(g, j);
     }
+    __syncthreads();
+    int base = lo;
+    for (; base + TILE <= hi; base += TILE) {
+        const int i0 = base + (int)threadIdx.x * N;
+        Vec<T> raw[kU];
+        uint8_t mk[kU][N];
+#pragma unroll
+        for (int q = 0; q < kU; q++) {
+            raw[q] = load_vec(x + i0 + q * STRIDE);
+            if (MASK) __builtin_memcpy(mk[q], mask + i0 + q * STRIDE, N);
+        }
+#pragma unroll
+        for (int q = 0; q < kU; q++) {
+            Vec<T> out;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const float xv = to_f32(raw[q].v[j]);
+                const bool on = !rg.none && !(MASK && mk[q][j] == 0) && !(xv == -INFINITY);
+                out.v[j] = (T)(on ? rg.at(xv) : 0.0f);
+            }
+            store_vec(dx + i0 + q * STRIDE, out);
+        }
+    }
+    for (int i = base + (int)threadIdx.x; i < hi; i += THREADS) {
+        const float xv = to_f32(x[i]);
+        const bool on = !rg.none && !(MASK && mask[i] == 0) && !(xv == -INFINITY);
+        dx[i] = (T)(on ? rg.at(xv) : 0.0f);
+    }
+    __syncthreads();
+    if (mine) dx[named] = (T)patch;
 }
 
 // ---- plans --------------------------------------------------------------------------------
@@ -975,24 +967,33 @@ size_t part_bytes(int rows, int splits, int top) {
 }
 
 constexpr int kMaxVocab = 1 << 30;
-// workgroups of a launch: threads of a grid are counted in 32 bits.  (Rows are counted in 64 bits by
-// the loops over them: the last workgroup's next row is up to twice their number.)
+// workgroups of a launch: threads of a grid are counted in 32 bits
 constexpr int64_t kMaxGroups = ((int64_t)1 << 32) / 256 - 1;
-int capped_groups(int64_t g, int threads = 256) {
-    const int64_t most = kMaxGroups / (threads / 256);
-    return (int)(g < most ? g : most);
-}
+int capped_groups(int64_t g) { return (int)(g < kMaxGroups ? g : kMaxGroups); }
 
 // one thread a row has no use for alternatives: 16 lanes find them together
 // (8: a vector of 16-bit logits)
 bool by_rows(int rows, int vocab, int top) { return rows >= kRowsFrom && vocab >= 8 && vocab <= kRowsMax && top == 0; }
-int rows_groups(int rows) { return capped_groups(((int64_t)rows + kRowsThreads - 1) / kRowsThreads); }
+int rows_groups(int rows) { return (int)(((int64_t)rows + kRowsThreads - 1) / kRowsThreads); }   // at most 2^31 threads
 size_t rows_lds(int vocab) { return (size_t)kRowsThreads * rows_pitch(vocab) * sizeof(float); }
+
+// launch(arguments, grid) for all rows, `per` of them a workgroup and as many a launch as it has
+// workgroups for.  (Loops over rows inside the kernels, in 64 bits, cost registers and instructions:
+// scores of 100 000 x 300 fp32 46 us instead of 38, the gradient of 1001 x 32 003 fp16 with a mask 47
+// instead of 38.)
+template <class Args, class Launch>
+void in_launches(Args a, int64_t per, Launch launch) {
+    const int64_t most = kMaxGroups * per;
+    for (int64_t row0 = 0; row0 < a.rows; row0 += most) {
+        const int64_t here = a.rows - row0 < most ? a.rows - row0 : most;
+        a.row0 = (int)row0;
+        launch(a, dim3((unsigned)((here + per - 1) / per)));
+    }
+}
 
 template <typename T, bool MASK>
 void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
     if (pl.kind == 0) {
-        const dim3 small(capped_groups(((int64_t)a.rows + 15) / 16)), wide(capped_groups(((int64_t)a.rows + 3) / 4));
         if (by_rows(a.rows, a.vocab, a.top)) {
             const dim3 grid(rows_groups(a.rows)), block(kRowsThreads);
             constexpr int PER_16 = 16 / Vec<T>::N;
@@ -1001,10 +1002,12 @@ void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
             else hipLaunchKernelGGL((k_logprobs_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
         } else {
             const int vectors = (a.vocab + Vec<T>::N - 1) / Vec<T>::N;   // 16 lanes up to 32 of them
-            if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_short<T, 16, 1, MASK>), small, dim3(256), 0, st, a);
-            else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
-            else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_short<T, 64, 1, MASK>), wide, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((k_logprobs_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+            in_launches(a, vectors <= 32 ? 16 : 4, [&](const LpArgs& b, dim3 grid) {
+                if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_short<T, 16, 1, MASK>), grid, dim3(256), 0, st, b);
+                else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_short<T, 16, 2, MASK>), grid, dim3(256), 0, st, b);
+                else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_short<T, 64, 1, MASK>), grid, dim3(256), 0, st, b);
+                else hipLaunchKernelGGL((k_logprobs_short<T, 64, 2, MASK>), grid, dim3(256), 0, st, b);
+            });
         }
     } else if (pl.kind == 1) {
         const dim3 grid(capped_groups(((int64_t)a.rows + 3) / 4));
@@ -1020,7 +1023,6 @@ void run_forward(const LpArgs& a, const LpPlan& pl, hipStream_t st) {
 template <typename T, bool MASK>
 void run_grad(const LpGradArgs& a, const LpPlan& pl, hipStream_t st) {
     if (pl.kind == 0) {
-        const dim3 small(capped_groups(((int64_t)a.rows + 15) / 16)), wide(capped_groups(((int64_t)a.rows + 3) / 4));
         if (by_rows(a.rows, a.vocab, a.top)) {
             const dim3 grid(rows_groups(a.rows)), block(kRowsThreads);
             constexpr int PER_16 = 16 / Vec<T>::N;
@@ -1029,18 +1031,25 @@ void run_grad(const LpGradArgs& a, const LpPlan& pl, hipStream_t st) {
             else hipLaunchKernelGGL((k_logprobs_grad_rows<T, 4 * PER_16, MASK>), grid, block, rows_lds(a.vocab), st, a);
         } else {
             const int vectors = (a.vocab + Vec<T>::N - 1) / Vec<T>::N;   // 16 lanes up to 32 of them
-            if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 1, MASK>), small, dim3(256), 0, st, a);
-            else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 2, MASK>), small, dim3(256), 0, st, a);
-            else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 1, MASK>), wide, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), wide, dim3(256), 0, st, a);
+            in_launches(a, vectors <= 32 ? 16 : 4, [&](const LpGradArgs& b, dim3 grid) {
+                if (vectors <= 16) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 1, MASK>), grid, dim3(256), 0, st, b);
+                else if (vectors <= 32) hipLaunchKernelGGL((k_logprobs_grad_short<T, 16, 2, MASK>), grid, dim3(256), 0, st, b);
+                else if (vectors <= 64) hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 1, MASK>), grid, dim3(256), 0, st, b);
+                else hipLaunchKernelGGL((k_logprobs_grad_short<T, 64, 2, MASK>), grid, dim3(256), 0, st, b);
+            });
         }
     } else {
-        const int64_t items = (int64_t)a.rows * a.splits;
-        if (a.x == a.dx)
-            hipLaunchKernelGGL((k_logprobs_grad<T, MASK, kInPlaceThreads>), dim3(capped_groups(items, kInPlaceThreads)),
-                               dim3(kInPlaceThreads), 0, st, a);
-        else
-            hipLaunchKernelGGL((k_logprobs_grad<T, MASK, 256>), dim3(capped_groups(items)), dim3(256), 0, st, a);
+        // a.splits workgroups a row
+        const bool in_place = a.x == a.dx;
+        const int threads = in_place ? kInPlaceThreads : 256;
+        const int64_t most = kMaxGroups / (threads / 256) / a.splits;
+        LpGradArgs b = a;
+        for (int64_t row0 = 0; row0 < a.rows; row0 += most) {
+            b.row0 = (int)row0;
+            const dim3 grid((unsigned)((a.rows - row0 < most ? a.rows - row0 : most) * a.splits));
+            if (in_place) hipLaunchKernelGGL((k_logprobs_grad<T, MASK, kInPlaceThreads>), grid, dim3(threads), 0, st, b);
+            else hipLaunchKernelGGL((k_logprobs_grad<T, MASK, 256>), grid, dim3(threads), 0, st, b);
+        }
     }
 }
 

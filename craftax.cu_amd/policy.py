@@ -560,7 +560,8 @@ def _rows_of(t, name):
     _need(t.is_cuda and t.dim() == 2 and t.dtype in _DTYPES,
           f"{name}: a [rows][vocab] fp32, bf16 or fp16 tensor on the GPU expected")
     _need(t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1), f"{name}: rows must be contiguous")
-    _need(max(t.shape) < 1 << 31, f"{name}: at most 2^31 - 1 rows and columns")   # the library's counts are C ints
+    if (t.shape[0] | t.shape[1]) >> 31:   # the library's counts are C ints
+        raise ValueError(f"{name}: at most 2^31 - 1 rows and columns")
     return t.data_ptr(), _DTYPES[t.dtype], t.stride(0)
 
 
@@ -644,7 +645,8 @@ def _matrices_of(t, name):
           f"{name}: a [rows][cols] or [batch][rows][cols] fp32, bf16 or fp16 tensor on the GPU expected")
     _need(t.shape[-2] > 0 and t.shape[-1] > 0 and (t.shape[-1] == 1 or t.stride(-1) == 1),
           f"{name}: rows must be contiguous and not empty")
-    _need(max(t.shape) < 1 << 31, f"{name}: at most 2^31 - 1 matrices, rows and columns")
+    if max(t.shape) >> 31:
+        raise ValueError(f"{name}: at most 2^31 - 1 matrices, rows and columns")
     batch, stride = (t.shape[0], t.stride(0)) if t.dim() == 3 else (1, 0)
     return t.data_ptr(), _DTYPES[t.dtype], t.stride(-2), stride, batch, t.shape[-2], t.shape[-1]
 
