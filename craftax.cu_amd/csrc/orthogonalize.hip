@@ -22,7 +22,7 @@
 //   P = 1  one fp16 product; X alone keeps its lo part, for the term a X.  Without it the
 //          rounding of X at every step is amplified by a (3.44) a step where singular values
 //          are small: 5e-3 of the norm measured instead of 1 to 2e-3.  A third of the matrix
-//          instructions (4096 x 4096 bf16: 1.46 ms, 3.56 with three), and only where the caller
+//          instructions (4096 x 4096 bf16: 1.46 ms, 3.53 with three), and only where the caller
 //          says so: what it loses, 7e-4 of the norm before the result is rounded, is not lost
 //          in a bf16 rounding (1.66e-3; together 1.80e-3).
 #include <utility>
@@ -787,8 +787,8 @@ __global__ __launch_bounds__(64 * kBlockWaves) void k_ortho_block(MulArgs g) {
 }
 
 // The parts of a tile of X X^T, added up in the order of the splits.  (A launch of its own: the
-// fences of a last-one-adds scheme inside the product cost 65 us a launch here, each writes back
-// an L2.)
+// fences of a last-one-adds scheme inside the product cost 65 to 86 us a launch here, each writes
+// back an L2.)
 template <int P>
 __global__ __launch_bounds__(256) void k_ortho_fold(MulArgs g) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -993,7 +993,7 @@ __global__ __launch_bounds__(256) void k_ortho_pair(MulArgs g) {
 // all steps run in one launch of one workgroup a matrix: the launches above cost 4 us each, the
 // work of one of them here is a fraction of one (all steps, fp32, launches / one workgroup each:
 // 1 x 32 x 32 50 / 20 us, 1 x 64 x 64 50 / 25, 1 x 64 x 256 57 / 44, 300 x 64 x 64 91 / 50,
-// 1000 x 32 x 128 238 / 94; bf16 1 x 128 x 128 50 / 41).  Bound by the chain of five barriers and
+// 1000 x 32 x 128 238 / 94; one product 1 x 128 x 128 50 / 41).  Bound by the chain of five barriers and
 // three products a step.  Operands are [32 values][rows][64 bytes] as in
 // k_ortho_pair.  A wavefront owns up to two 32 x 32 blocks and keeps their X in fp32 registers
 // (C layout: column n32, rows 8 q + 4 half + e), so the a X term needs no lo part.
@@ -1233,7 +1233,7 @@ int tile_for(bool sym, int rows, int cols, int batch) {
 }
 // k_ortho_block while its blocks find a CU each (two or four: 700 x 700 fp32, all steps, 130 us
 // instead of 120) and a wavefront's share of the K axis is short (of 126 stages: 250 x 2000 fp32
-// 124 us, split over workgroups 118; of 63: bf16 91 us, split 99)
+// 124 us, split over workgroups 118; of 63: with one product 91 us, split 99)
 bool in_blocks(bool sym, int rows, int cols, int batch, int stages) {
     const int64_t ti = rows / 32, tj = cols / 32;
     return (sym ? ti * (ti + 1) / 2 : ti * tj) * batch <= 256 && stages <= 100;
@@ -1265,8 +1265,8 @@ Plan make_plan(int batch, int rows, int cols, int products) {
     // X X^T of few small tiles with many stages: the stages shared out until about two workgroups a
     // CU run, none with less than 16 stages of 64 values (all steps, fp32, unsplit / 8 / 16 / 32 stages:
     // 1 x 64 x 2048: 101 / 75 / 78 / 88 us, 1 x 250 x 4000: 200 / 139 / 136 / 149,
-    // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000 bf16: 80 / 86 / 80 / 80).  Two workgroups
-    // a tile on half of the CUs gain nothing (1 x 1000 x 2731 bf16: 200 us unsplit, 219 split).
+    // 1 x 500 x 4500: 264 / 215 / 213 / 199; 1 x 250 x 1000, one product: 80 / 86 / 80 / 80).  Two workgroups
+    // a tile on half of the CUs gain nothing (1 x 1000 x 2731, one product: 200 us unsplit, 219 split).
     p.splits = 1;
     if (tile_for(true, p.mp, p.mp, batch) == 1 && !in_blocks(true, p.mp, p.mp, batch, p.ldn / 32)) {
         const int64_t nt = p.mp / 64, tiles = nt * (nt + 1) / 2 * batch;
@@ -1295,7 +1295,7 @@ void run_mul(MulArgs g, int batch, hipStream_t st) {
     // Workgroups go to the eight XCDs in turn.  Where the CUs take more than one each, an XCD takes a
     // run of tiles of neighbouring rows and columns, which share panels in its L2; one tile a CU is
     // faster in plain order, where an XCD keeps to one row's panel (all steps, runs / plain order:
-    // 2048 x 8192 bf16 998 / 1030 us, 1000 x 2731 fp32 292 / 302; 2 x 500 x 1000 fp32 160 / 135,
+    // 2048 x 8192 one product 998 / 1030 us, 1000 x 2731 fp32 292 / 302; 2 x 500 x 1000 fp32 160 / 135,
     // 700 x 700 fp32 138 / 124).
     g.runs = !g.by_xcd && (int64_t)tiles * F * batch > 256;
     g.row_len = SYM ? g.tiles_i + 1 : g.runs ? 4 * tiles_j : g.tiles_i;
@@ -1332,7 +1332,7 @@ void run_mul(const MulArgs& g, int batch, hipStream_t st) {
 // The pair kernel reads all of A in every workgroup: worth it up to 128 KiB of A (m = 128 with
 // P = 3, 256 with P = 1) and while one or two rounds of workgroups do.  All five steps, with it and
 // without: 1 x 128 x 512 fp32 68 / 80 us, 1 x 192 x 800 fp32 95 / 95, 1 x 256 x 843 fp32 114 / 104,
-// the same in bf16 78 / 84.
+// the same with one product 78 / 84.
 template <int P>
 bool use_pair(const Work& w, int batch) {
     return w.mp <= (P == 3 ? 128 : 256) && (int64_t)(w.mp / 32) * ((w.np + 127) / 128) * batch <= 512;
