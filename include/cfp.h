@@ -456,10 +456,11 @@ int cfp_token_logprobs_grad(const void* d_logits, int dtype, int64_t ld, int row
  * beside it, an overlap is an error.  coefs: host [steps][3], NULL = (3.4445, -4.7750, 2.0315)
  * for every step; the iterates must keep |X| < 64 and |A|, |B| < 256.
  * products: 3 (or 0) = three fp16 matrix products per product (1e-6 of the result's norm from the
- * 64-bit result, as fp32 has), 1 = one (up to 2e-3, in a third of the time).  Entries of X are held
- * to 2^-35 at best: a |G| far below eps, whose result is small, leaves an error of up to 2e-8
- * sqrt(rows cols) after five standard steps.  Sums are fp32, the norm is 64-bit.  A zero matrix
- * gives zeros; NaN or infinity in a matrix makes all of it NaN.
+ * 64-bit result, a few 1e-5 for matrices nearly of one direction, as fp32 has), 1 = one (up to
+ * 2e-3, in a third of the time).  Entries of X are held to 2^-35 at best: a |G| far below eps,
+ * whose result is small, leaves an error of up to 2e-8 sqrt(rows cols) after five standard steps.
+ * Sums are fp32, the norm is 64-bit.  A zero matrix gives zeros; NaN or infinity in a matrix makes
+ * all of it NaN.
  * d_work: cfp_orthogonalize_workspace(batch, rows, cols, products) bytes (products 1 or 3),
  * 256-byte aligned (may be NULL where that is 0: matrices that fit into one workgroup); calls that
  * may overlap need one each. */

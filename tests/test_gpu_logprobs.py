@@ -626,3 +626,35 @@ def test_sizes_past_the_library_counts_are_refused(pkg, cuda):
         pkg.policy.orthogonalize(x, out=x)
     del x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [("f32", 300, 43), ("bf16", 3, 60001), ("f16", 16500, 42)])
+def test_in_place_from_a_graph(pkg, cuda, dtype, rows, vocab):
+    """Scores and the gradient in their place, captured and replayed on new logits between eager work."""
+    torch = _torch()
+    pol = pkg.policy
+    x, tok = make(cuda, dtype, rows, vocab, ld=vocab + 1, seed=41)
+    buf = torch.full((rows, vocab + 1), 9.0, dtype=x.dtype, device=cuda)
+    y = buf[:, :vocab]
+    g = torch.randn(rows, generator=torch.Generator().manual_seed(4)).to(cuda)
+
+    def both(t, out):
+        r = pol.token_logprobs(t, tok, stats=True)
+        pol.token_logprobs_backward(t, tok, r.stats, g_logprobs=g, g_entropy=g, out=out)
+        return r.logprobs
+
+    y.copy_(x)
+    both(y, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lp = both(y, y)
+    for rep in range(4):
+        x, _ = make(cuda, dtype, rows, vocab, ld=vocab + 1, seed=42 + rep)
+        want = torch.empty_like(y)
+        want_lp = both(x, want)
+        y.copy_(x)
+        lp.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(lp, want_lp) and buf[:, vocab].eq(9).all()

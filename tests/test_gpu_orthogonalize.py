@@ -434,3 +434,61 @@ def test_errors_are_those_of_the_formats(pkg, cuda, products, rows, cols, fall):
     there = (in_the_formats(g, products) - want).norm()
     here = (pkg.policy.orthogonalize(g, products=products).double().cpu() - want).norm()
     assert here <= (1.5 if products == 1 else 3.0) * there + 2.0 ** -24 * want.norm(), (here / want.norm(), there / want.norm())
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 65536, 1), (1, 1, 65536), (1, 65536, 40), (1, 200, 65536)])
+def test_largest_sides_and_batches(pkg, cuda, batch, rows, cols):
+    g = gradient(cuda, batch, rows, cols, seed=12, fall=0.0)
+    got = pkg.policy.orthogonalize(g)
+    assert off(got, reference(g)) <= tolerance("f32", 3, g.shape)
+    assert off(pkg.policy.orthogonalize(g, products=1), reference(g)) <= tolerance("f32", 1, g.shape)
+
+
+@pytest.mark.parametrize("products", [1, 3])
+def test_the_largest_batch(pkg, cuda, products):
+    """65 535 random matrices of 3 x 2.  Among so many some are nearly of one direction, and the bound is
+    grown()'s for each: four roundings a step, of 2^-23 (three products) or 2^-12 (one) of X, amplified by
+    3.4445 a step that follows.  (tolerance() holds for matrices that use all their directions alike.)"""
+    g = gradient(cuda, 65535, 3, 2, seed=12, fall=0.0)
+    x = [reference(g, t).flatten(1).norm(dim=1) for t in range(5)]
+    bound = sum(4 * 2.0 ** (-12 if products == 1 else -23) * x[t] * QUINTIC[0] ** (5 - t) for t in range(5))
+    error = (pkg.policy.orthogonalize(g, products=products).double().cpu() - reference(g)).flatten(1).norm(dim=1)
+    assert (error <= bound).all(), (error / bound).max().item()
+    assert error.median() <= tolerance("f32", products, g.shape)
+
+
+@pytest.mark.parametrize("cols", [50, 400])
+def test_rows_far_apart(pkg, cuda, cols):
+    """Rows 2^30 + 9 entries apart: the third begins 2^33 bytes in."""
+    torch = _torch()
+    torch.cuda.empty_cache()
+    ld = (1 << 30) + 9
+    small = [gradient(cuda, 1, 3, cols, seed=60 + k)[0] for k in range(3)]
+    want_o = pkg.policy.orthogonalize(small[1])
+    store = torch.empty(3 * ld, device=cuda)
+    at = lambda k: torch.as_strided(store, (3, cols), (ld, 1), k * cols)
+    for k in range(3):
+        at(k).copy_(small[k])
+    pkg.policy.orthogonalize(at(1), out=at(3))
+    assert torch.equal(at(3), want_o)
+    pkg.policy.muon_update(*(at(k) for k in range(3)), 0.1)
+    pkg.policy.muon_update(*small, 0.1)
+    for k in range(3):
+        assert torch.equal(at(k), small[k])
+    del store
+    torch.cuda.empty_cache()
+
+
+def test_many_matrices_that_need_a_workspace(pkg, cuda):
+    """20 000 matrices of 128 x 160: the first, the middle and the last as in 64 bits, in the batch's plan."""
+    torch = _torch()
+    torch.cuda.empty_cache()
+    few = gradient(cuda, 3, 128, 160, seed=70)
+    g = few.repeat(6667, 1, 1)[:20000]
+    got = pkg.policy.orthogonalize(g)
+    want = reference(few)
+    for k in (0, 10000, 19999):
+        assert off(got[k], want[k % 3]) <= tolerance("f32", 3, few.shape)
+    assert torch.equal(got[:3].repeat(6667, 1, 1)[:20000], got)
+    del g, got
+    torch.cuda.empty_cache()
