@@ -43,9 +43,10 @@ def check_no_scratch(remarks):
 # the operations the source issues between a load and its use; how many wavefronts share a
 # SIMD decides how far ahead those loads have to be issued (the forward kernels are written
 # for one, respectively two, wavefronts per SIMD; the sweep for at least four, its
-# __launch_bounds__; the Newton-Schulz products for one or two, as their LDS rings fit), and a jump in registers is how a compiler change that re-orders or
-# duplicates those loads shows first.  (kernel name part, VGPRs allowed, AGPRs allowed,
-# occupancy [waves/SIMD] lowest, highest)
+# __launch_bounds__; the Newton-Schulz products for one or two, as their LDS rings fit), and
+# a jump in registers is how a compiler change that re-orders or duplicates those loads shows
+# first.  (kernel name part, VGPRs allowed, AGPRs allowed, occupancy [waves/SIMD] lowest,
+# highest)
 COUNTED_WAIT_BUDGET = (
     ("k_policy_forwardI", 256, 160, 1, 1),
     ("k_policy_forward_t16I", 192, 0, 2, 2),

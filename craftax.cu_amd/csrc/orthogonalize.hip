@@ -23,8 +23,8 @@
 //          rounding of X at every step is amplified by a (3.44) a step where singular values
 //          are small: 5e-3 of the norm measured instead of 1 to 2e-3.  A third of the matrix
 //          instructions (4096 x 4096 bf16: 1.46 ms, 3.53 with three), and only where the caller
-//          says so: what it loses, 7e-4 of the norm before the result is rounded, is not lost
-//          in a bf16 rounding (1.66e-3; together 1.80e-3).
+//          says so: what it loses, 7e-4 of the norm before the result is rounded, shows beside
+//          a bf16 rounding (1.66e-3; together 1.80e-3).
 #include <utility>
 
 #include "cfp_internal.h"
